@@ -29,6 +29,13 @@ class TsdfThresholds(C.Structure):
     _fields_ = [(n, C.c_float) for n in ("trunc", "thr_neg", "thr_pos", "max_depth_h", "min_depth", "depth_range")]
 
 
+class PlaneDesc(C.Structure):
+    """struct dt_plane_desc (include/doubletake_hip.h)."""
+    _fields_ = [("b", C.c_int), ("d", C.c_int), ("h", C.c_int), ("w", C.c_int), ("dtype", C.c_int), ("top", C.c_int),
+                ("scale", C.c_float), ("pad", C.c_int), ("vol_stride", C.c_int64 * 4), ("mask_stride", C.c_int64 * 4),
+                ("planes_stride", C.c_int64 * 4), ("grad_stride", C.c_int64 * 4)]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _L = C.c_int64
@@ -62,6 +69,9 @@ SIGNATURES = {
     "dt_cv_dot_simple_f32": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "dt_cv_lowest_cost_f32": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "dt_cv_overall_mask_u8": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "dt_cv_plane_log_probs": (_I, [C.POINTER(PlaneDesc)] + [_P] * 13),
+    "dt_cv_plane_log_probs_grad": (_I, [C.POINTER(PlaneDesc)] + [_P] * 13),
+    "dt_cv_nearest_planes_f32": (_I, [_P, _P, C.POINTER(_L), _I, _I, _I, _I, _P, _P]),
     "dt_conv_pack_floats": (_L, [_I, _I, _I]),
     "dt_conv_pack_f32": (_I, [_P, _P, _I, _I, _I, _P]),
     "dt_conv2d_f32": (_I, [C.POINTER(ConvDesc), _P, _P, _P, _P, _P, _P, _P, _P]),

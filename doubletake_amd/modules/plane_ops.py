@@ -1,0 +1,192 @@
+"""The plane-sweep volume as a distribution over depth planes (csrc/cv_plane_stats.hip).
+
+A volume [b, D, h, w] scores D depth planes per pixel.  The reference takes one thing from it outside the networks, the plane of
+the highest score (argmax + gather, modules/cost_volume.py:355-361: ``lowest_cost``).  Read as logits the same scores also say how
+probable any other depth is and how sure the matching is:
+
+    plane_log_probs  log probability of a given plane, entropy, normaliser and the most probable planes of every pixel; differentiable
+    nearest_planes   the plane index a metric depth falls on -- what a predicted, rendered or measured depth map is scored by
+
+``CostVolumeManager.plane_statistics`` puts the two together; ``model.enable_plane_statistics()`` adds the result to the model's
+outputs.  No CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _abi
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+#: most alternatives per pixel (DT_PLANE_MAX_TOP)
+MAX_TOP = 8
+
+
+class PlaneLogProbs(NamedTuple):
+    """What ``plane_log_probs`` returns; entries that were not asked for are None.  Real-valued entries are float32."""
+    log_prob_bhw: Optional[torch.Tensor]        # of the given plane; 0 where it is outside 0..D-1
+    entropy_bhw: torch.Tensor                   # nats
+    log_sum_bhw: torch.Tensor                   # log of the sum of exp(scale * score)
+    top_log_prob_bkhw: Optional[torch.Tensor]   # descending
+    top_plane_bkhw: Optional[torch.Tensor]      # int64, as indices_to_disparity takes them; -1 where there is none
+    top_depth_bkhw: Optional[torch.Tensor]
+
+
+def _require_gpu(t, name):
+    if not t.is_cuda:
+        raise _abi.DoubletakeHipError(f"{name} is on {t.device}; doubletake_amd plane statistics only run on a ROCm GPU (no CPU fallback)")
+
+
+def _broadcast(t, shape, device, name):
+    """``t`` as a view of ``shape`` = (b, D, h, w) with stride 0 along the axes it is broadcast over."""
+    if t.dim() != 4 or any(n != m and n != 1 for n, m in zip(t.shape, shape)):
+        raise ValueError(f"{name} {tuple(t.shape)} does not broadcast to {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    return t.expand(shape)
+
+
+def _desc(vol, top, scale, mask, planes, grad=None):
+    d = _abi.PlaneDesc()
+    d.b, d.d, d.h, d.w = vol.shape
+    d.dtype, d.top, d.scale = _DTYPES[vol.dtype], top, scale
+    d.vol_stride[:] = vol.stride()
+    if mask is not None:
+        d.mask_stride[:] = mask.stride()
+    if planes is not None:
+        d.planes_stride[:] = planes.stride()
+    if grad is not None:
+        d.grad_stride[:] = grad.stride()
+    return d
+
+
+def _forward(vol, plane, top, scale, mask, planes, for_grad):
+    b, _, h, w = vol.shape
+    f32 = lambda *shape: torch.empty(shape, device=vol.device, dtype=torch.float32)
+    ent, lsum = f32(b, h, w), f32(b, h, w)
+    lp = f32(b, h, w) if plane is not None else None
+    tlp = f32(b, top, h, w) if top else None
+    tpl = torch.empty((b, top, h, w), device=vol.device, dtype=torch.int64) if top else None
+    tdep = f32(b, top, h, w) if planes is not None else None
+    rmax, rlog = (f32(b, h, w), f32(b, h, w)) if for_grad else (None, None)
+    if b * h * w:
+        p = _abi.ptr
+        _abi.check(_abi.lib().dt_cv_plane_log_probs(
+            C.byref(_desc(vol, top, scale, mask, planes)), p(vol), p(mask), p(plane), p(planes), p(lp), p(ent), p(lsum), p(tlp), p(tpl),
+            p(tdep), p(rmax), p(rlog), _abi.current_stream(vol.device)), "dt_cv_plane_log_probs")
+    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rmax, rlog
+
+
+class _PlaneLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, vol, plane, top, scale, mask, planes):
+        out, rmax, rlog = _forward(vol, plane, top, scale, mask, planes, True)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*[t for t in (out.top_plane_bkhw, out.top_depth_bkhw) if t is not None])
+        ctx.save_for_backward(vol, plane, mask, out.entropy_bhw, out.top_plane_bkhw, rmax, rlog)
+        ctx.top, ctx.scale = top, scale
+        return tuple(out)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
+        vol, plane, mask, ent, tpl, rmax, rlog = ctx.saved_tensors
+        dense = lambda g: None if g is None else g.to(torch.float32).contiguous()
+        g_lp, g_ent, g_lsum, g_top = dense(g_lp), dense(g_ent), dense(g_lsum), dense(g_top)
+        grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
+        if vol.numel():
+            p = _abi.ptr
+            _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
+                C.byref(_desc(vol, ctx.top, ctx.scale, mask, None, grad)), p(vol), p(mask), p(plane), p(ent), p(tpl), p(rmax), p(rlog),
+                p(g_lp), p(g_ent), p(g_lsum), p(g_top), p(grad), _abi.current_stream(vol.device)), "dt_cv_plane_log_probs_grad")
+        return grad, None, None, None, None, None
+
+
+def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=None, depth_planes_bdhw=None) -> PlaneLogProbs:
+    """Log probabilities over the depth planes of a volume [b, D, h, w], in one pass over it.
+
+    volume_bdhw: float32, float16 or bfloat16 scores in any layout (NCHW, channels_last, slices); statistics are float32.
+    plane_bhw: plane indices [b, h, w] (int64 or int32) whose log probability is wanted; one outside 0..D-1 (-1: no depth there)
+        scores 0 and takes no part in the gradient.
+    top: how many of the most probable planes to return, 0..min(D, 8); equal scores in the order of their planes.
+    scale: factor on the scores in front of the softmax (inverse temperature), a positive number.
+    mask_bdhw: bool, broadcastable to the volume; False leaves a plane out, whatever the volume holds there.  A pixel without a
+        visible plane of a score above -inf has entropy 0, log_sum and log_prob -inf, no alternatives (plane -1, log probability -inf,
+        depth 0) and gradient 0.
+    depth_planes_bdhw: float32 depths of the planes, broadcastable to the volume (what the managers return): the alternatives' depths
+        are returned too.
+
+    Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice): the gradient has the volume's
+    type and layout.  A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on
+    the current stream and can be captured into a graph; capture a backward pass only together with its forward pass."""
+    vol = volume_bdhw
+    if vol.dim() != 4:
+        raise ValueError(f"volume_bdhw must be [b, D, h, w], got {tuple(vol.shape)}")
+    if vol.dtype not in _DTYPES:
+        raise ValueError(f"volume_bdhw is {vol.dtype}; float32, float16 and bfloat16 are supported")
+    b, D, h, w = vol.shape
+    if D < 1:
+        raise ValueError("volume_bdhw has no planes")
+    if b * h * w >= 2**31 - 1:
+        raise ValueError(f"volume_bdhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
+    top = int(top)
+    if not 0 <= top <= min(D, MAX_TOP):
+        raise ValueError(f"top={top} not in 0..{min(D, MAX_TOP)}")
+    scale = float(scale)
+    if not (0.0 < scale <= 3.4e38):
+        raise ValueError(f"scale={scale} must be positive and finite")
+    plane = plane_bhw
+    if plane is not None:
+        if plane.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"plane_bhw is {plane.dtype}; int64 or int32 plane indices expected")
+        if plane.shape != (b, h, w):
+            raise ValueError(f"plane_bhw {tuple(plane.shape)} does not match the volume's pixels {(b, h, w)}")
+        if plane.device != vol.device:
+            raise ValueError(f"plane_bhw is on {plane.device}, expected {vol.device}")
+        plane = plane.to(torch.int64).contiguous()
+    mask = mask_bdhw
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise ValueError(f"mask_bdhw is {mask.dtype}; bool expected")
+        mask = _broadcast(mask, vol.shape, vol.device, "mask_bdhw")
+    planes = depth_planes_bdhw
+    if planes is not None:
+        if not top:
+            raise ValueError("depth_planes_bdhw gives the alternatives their depths: it goes with top > 0")
+        if planes.dtype != torch.float32:
+            raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
+        planes = _broadcast(planes, vol.shape, vol.device, "depth_planes_bdhw")
+    _require_gpu(vol, "volume_bdhw")
+    if vol.requires_grad and torch.is_grad_enabled():
+        return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes))
+    return _forward(vol, plane, top, scale, mask, planes, False)[0]
+
+
+@torch.no_grad()
+def nearest_planes(depth_bhw, depth_planes_bdhw):
+    """int64 [b, h, w]: index of the depth plane nearest to each depth (absolute difference, the lowest index of equally near ones), the depths taken in float32;
+    -1 where the depth is not finite or not positive (holes of a sensor's map, a renderer's background).  depth_planes_bdhw is
+    float32 and broadcastable to [b, D, h, w] (what the cost-volume managers return)."""
+    depth, planes = depth_bhw, depth_planes_bdhw
+    if depth.dim() != 3:
+        raise ValueError(f"depth_bhw must be [b, h, w], got {tuple(depth.shape)}")
+    if not depth.is_floating_point():
+        raise ValueError(f"depth_bhw is {depth.dtype}; metric depths are floating point")
+    if planes.dim() != 4 or planes.shape[1] < 1:
+        raise ValueError(f"depth_planes_bdhw must be [b, D, h, w], got {tuple(planes.shape)}")
+    if planes.dtype != torch.float32:
+        raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
+    b, h, w = depth.shape
+    D = planes.shape[1]
+    if b * h * w >= 2**31 - 1:
+        raise ValueError(f"depth_bhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
+    planes = _broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw")
+    _require_gpu(depth, "depth_bhw")
+    depth = depth.to(torch.float32).contiguous()
+    out = torch.empty((b, h, w), device=depth.device, dtype=torch.int64)
+    if out.numel():
+        _abi.check(_abi.lib().dt_cv_nearest_planes_f32(_abi.ptr(depth), _abi.ptr(planes), (C.c_int64 * 4)(*planes.stride()), b, D, h, w,
+                                                       _abi.ptr(out), _abi.current_stream(depth.device)), "dt_cv_nearest_planes_f32")
+    return out

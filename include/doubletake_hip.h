@@ -204,6 +204,54 @@ int dt_cv_overall_mask_u8(const float* params, const float* depth_planes_bdhw, u
                           int per_view, int batch, int num_src, int h, int w, int num_planes,
                           dt_stream_t s);
 
+/* ---- the volume as a distribution over depth planes ------------------------------------
+ * The D plane scores of a pixel read as logits.  With y_d = scale * x_d over the planes the mask leaves visible, m = max x and
+ * s = sum_d exp(scale (x_d - m)):
+ *   log_sum = scale m + ln s;   lp_d = scale (x_d - m) - ln s;   entropy = -sum_d exp(lp_d) lp_d
+ * No reference counterpart: dt_cv_lowest_cost_f32's argmax (modules/cost_volume.py:355-361) is the most probable plane of the same
+ * distribution.  Statistics are fp32 whatever the volume's type.  Edges, the same for every entry point below:
+ *   - masked planes may hold anything (NaN, infinities); a score of -inf is a plane without probability;
+ *   - a pixel without any probability: log_sum = log_prob = -inf, entropy = 0, no alternatives, gradient 0;
+ *   - a visible NaN or +inf makes the pixel's real-valued outputs NaN (the order of the alternatives stays defined: NaN first);
+ *   - a given plane outside 0..d-1 scores nothing: log_prob = 0, no gradient;
+ *   - equal scores: the lowest plane first; alternatives beyond the planes with probability: plane -1, log prob -inf, depth 0. */
+enum { DT_VOL_F32 = 0, DT_VOL_F16 = 1, DT_VOL_BF16 = 2 };
+#define DT_PLANE_MAX_TOP 8
+
+typedef struct dt_plane_desc {
+  int b, d, h, w;             /* extents of the volume; b * h * w < 2^31 */
+  int dtype;                  /* DT_VOL_*: type of the volume and of its gradient */
+  int top;                    /* alternatives per pixel, 0..min(d, DT_PLANE_MAX_TOP) */
+  float scale;                /* inverse temperature, > 0 and finite */
+  int pad;
+  int64_t vol_stride[4];      /* elements between neighbours along b, d, y, x: any layout */
+  int64_t mask_stride[4];     /* bytes, likewise; 0 along a broadcast axis */
+  int64_t planes_stride[4];   /* elements of the depth planes, likewise */
+  int64_t grad_stride[4];     /* elements of the gradient written by ..._grad; the other call ignores it */
+} dt_plane_desc;
+
+/* Statistics of every pixel in one pass over the volume.  mask (1 byte per plane, 0 = not visible), plane_bhw and depth_planes may
+ * be NULL; depth_planes is read for the alternatives' depths only.  Outputs are dense: log_prob (with plane_bhw only), entropy and
+ * log_sum [b,h,w]; top_log_prob, top_plane and (with depth_planes) top_depth [b,top,h,w]; row_max and row_log [b,h,w] (both or
+ * neither) are m and ln s, what ..._grad needs.  Any output but entropy and log_sum may be NULL where it is not wanted. */
+int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint8_t* mask, const int64_t* plane_bhw,
+                          const float* depth_planes, float* log_prob, float* entropy, float* log_sum, float* top_log_prob,
+                          int64_t* top_plane, float* top_depth, float* row_max, float* row_log, dt_stream_t s);
+/* Gradient of the volume for gradients of the outputs above (each NULL where there is none; dense, shaped like its output):
+ *   dx_d = scale [ sum of the gradients that meet plane d (given plane, alternatives)
+ *                  + p_d (g_log_sum - g_log_prob - sum g_top) - g_entropy p_d (lp_d + entropy) ]
+ * mask, plane_bhw, entropy, top_plane, row_max and row_log are those of the forward call.  Every element of the gradient is
+ * written (0 for masked planes). */
+int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const uint8_t* mask, const int64_t* plane_bhw,
+                               const float* entropy, const int64_t* top_plane, const float* row_max, const float* row_log,
+                               const float* g_log_prob, const float* g_entropy, const float* g_log_sum, const float* g_top_log_prob,
+                               void* grad_volume, dt_stream_t s);
+/* The plane a metric depth falls on: argmin_d |depth - planes_d| per pixel (differences in 64 bits: exact), the lowest plane of
+ * equal ones; -1 where the depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x;
+ * 0 along a broadcast axis); a NaN plane is never the nearest. */
+int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
+                             int w, int64_t* plane_bhw, dt_stream_t s);
+
 /* ---- conv stacks (cost-volume encoder / depth decoders) --------------------------------
  * One implicit-GEMM primitive on NHWC fp32 tensors (fp32 MFMA):
  *   out[n,y,x,co] = act( bias[co] + sum_{ky,kx,ci} W[co,ky,kx,ci] * in[n, y*stride+ky-pad,

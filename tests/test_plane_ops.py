@@ -1,0 +1,164 @@
+"""plane_ops on the CPU: every refusal comes before a launch, and the 64-bit form the GPU tests compare with is itself checked
+against torch's log_softmax and against differences."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import plane_ref as ref
+from doubletake_amd import _abi
+from doubletake_amd.modules import plane_ops
+
+
+def _vol(b=2, D=5, h=3, w=4, dtype=torch.float32):
+    return torch.zeros(b, D, h, w, dtype=dtype)
+
+
+def _refusals():
+    v = _vol()
+    i = torch.zeros(2, 3, 4, dtype=torch.int64)
+    m = torch.ones(2, 5, 3, 4, dtype=torch.bool)
+    p = torch.ones(2, 5, 3, 4)
+    return {
+        "3-D volume": (v[0], {}),
+        "double volume": (v.double(), {}),
+        "integer volume": (v.long(), {}),
+        "no planes": (v[:, :0], {}),
+        "top over D": (v, dict(top=6)),
+        "top over 8": (_vol(D=20), dict(top=9)),
+        "top negative": (v, dict(top=-1)),
+        "scale zero": (v, dict(scale=0.0)),
+        "scale negative": (v, dict(scale=-1.0)),
+        "scale nan": (v, dict(scale=math.nan)),
+        "scale inf": (v, dict(scale=math.inf)),
+        "plane float": (v, dict(plane_bhw=i.float())),
+        "plane shape": (v, dict(plane_bhw=i[:, None])),
+        "plane size": (v, dict(plane_bhw=i[:1])),
+        "mask type": (v, dict(mask_bdhw=m.float())),
+        "mask dims": (v, dict(mask_bdhw=m[0])),
+        "mask size": (v, dict(mask_bdhw=m[:, :4])),
+        "planes without top": (v, dict(depth_planes_bdhw=p)),
+        "planes type": (v, dict(depth_planes_bdhw=p.double(), top=1)),
+        "planes size": (v, dict(depth_planes_bdhw=p[:, :, :2], top=1)),
+    }
+
+
+@pytest.mark.parametrize("name", sorted(_refusals()))
+def test_plane_log_probs_refuses(name):
+    vol, kw = _refusals()[name]
+    with pytest.raises(ValueError):
+        plane_ops.plane_log_probs(vol, **kw)
+
+
+def test_too_many_pixels_are_refused():
+    big = torch.zeros(1).expand(2, 3, 1 << 15, 1 << 15)
+    with pytest.raises(ValueError, match="pixels"):
+        plane_ops.plane_log_probs(big)
+    with pytest.raises(ValueError, match="pixels"):
+        plane_ops.nearest_planes(big[:, 0], torch.ones(1, 3, 1, 1))
+
+
+def test_no_cpu_fallback():
+    with pytest.raises(_abi.DoubletakeHipError):
+        plane_ops.plane_log_probs(_vol())
+    with pytest.raises(_abi.DoubletakeHipError):
+        plane_ops.nearest_planes(torch.ones(2, 3, 4), torch.ones(2, 5, 1, 1))
+
+
+@pytest.mark.parametrize("depth,planes", [
+    (torch.ones(2, 1, 3, 4), torch.ones(2, 5, 1, 1)),
+    (torch.ones(2, 3, 4, dtype=torch.int64), torch.ones(2, 5, 1, 1)),
+    (torch.ones(2, 3, 4), torch.ones(2, 5)),
+    (torch.ones(2, 3, 4), torch.ones(2, 0, 1, 1)),
+    (torch.ones(2, 3, 4), torch.ones(2, 5, 1, 1, dtype=torch.float64)),
+    (torch.ones(2, 3, 4), torch.ones(3, 5, 1, 1)),
+    (torch.ones(2, 3, 4), torch.ones(2, 5, 3, 3)),
+])
+def test_nearest_planes_refuses(depth, planes):
+    with pytest.raises(ValueError):
+        plane_ops.nearest_planes(depth, planes)
+
+
+def _desc(**kw):
+    d = _abi.PlaneDesc()
+    vals = dict(b=1, d=4, h=2, w=2, dtype=0, top=0, scale=1.0)
+    vals.update(kw)
+    for k, v in vals.items():
+        setattr(d, k, v)
+    return d
+
+
+def _call(d, **kw):
+    a = dict(volume=16, mask=None, plane=None, planes=None, log_prob=None, entropy=16, log_sum=16, tlp=None, tpl=None, tdep=None,
+             rmax=None, rlog=None)
+    a.update(kw)
+    return _abi.lib().dt_cv_plane_log_probs(C.byref(d) if d is not None else None, *a.values(), None)
+
+
+def _call_grad(d, **kw):
+    a = dict(volume=16, mask=None, plane=None, entropy=16, tpl=None, rmax=16, rlog=16, g_lp=None, g_ent=None, g_lsum=None, g_top=None,
+             grad=16)
+    a.update(kw)
+    return _abi.lib().dt_cv_plane_log_probs_grad(C.byref(d) if d is not None else None, *a.values(), None)
+
+
+@pytest.mark.parametrize("bad", [dict(b=0), dict(d=0), dict(h=-1), dict(w=0), dict(dtype=3), dict(dtype=-1), dict(top=5), dict(top=9, d=20),
+                                 dict(top=-1), dict(scale=0.0), dict(scale=-2.0), dict(scale=math.inf), dict(scale=math.nan),
+                                 dict(b=1 << 15, h=1 << 15, w=2)])
+def test_abi_refuses_descriptors(bad):
+    assert _call(_desc(**bad)) != 0 and _abi.lib().dt_last_error()
+    assert _call_grad(_desc(**bad)) != 0
+
+
+def test_abi_refuses_pointers():
+    assert _call(None) != 0 and _call_grad(None) != 0
+    for kw in (dict(volume=None), dict(entropy=None), dict(log_sum=None), dict(plane=16), dict(log_prob=16), dict(rmax=16),
+               dict(rlog=16), dict(tdep=16), dict(tdep=16, planes=16)):
+        assert _call(_desc(), **kw) != 0, kw
+    assert _call(_desc(top=2)) != 0 and _call(_desc(top=2), tlp=16) != 0
+    for kw in (dict(volume=None), dict(entropy=None), dict(rmax=None), dict(rlog=None), dict(grad=None), dict(g_lp=16),
+               dict(g_top=16), dict(g_top=16, tpl=16)):
+        assert _call_grad(_desc(), **kw) != 0, kw
+    L, st = _abi.lib(), (C.c_int64 * 4)(4, 1, 0, 0)
+    for args in ((None, 16, st, 1, 4, 2, 2, 16), (16, None, st, 1, 4, 2, 2, 16), (16, 16, None, 1, 4, 2, 2, 16), (16, 16, st, 1, 4, 2, 2, None),
+                 (16, 16, st, 0, 4, 2, 2, 16), (16, 16, st, 1, 0, 2, 2, 16), (16, 16, st, 1 << 15, 4, 1 << 15, 2, 16)):
+        assert L.dt_cv_nearest_planes_f32(*args, None) != 0, args
+
+
+def test_reference_form_matches_log_softmax():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 9, 4, 5, generator=g, dtype=torch.float64)
+    idx = torch.randint(0, 9, (2, 4, 5), generator=g)
+    r = ref.stats(x, idx, top=3, scale=0.5)
+    lp = torch.log_softmax(x * 0.5, 1)
+    assert torch.allclose(r["log_prob"], lp.gather(1, idx[:, None])[:, 0], atol=1e-14)
+    assert torch.allclose(r["entropy"], -(lp.exp() * lp).sum(1), atol=1e-14)
+    assert torch.allclose(r["log_sum"], torch.logsumexp(x * 0.5, 1), atol=1e-14)
+    v, i = torch.topk(lp, 3, dim=1)
+    assert torch.equal(r["top_plane"], i) and torch.allclose(r["top_log_prob"], v, atol=1e-14)
+
+
+def test_reference_gradient_matches_autograd_and_differences():
+    g = torch.Generator().manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    x, idx = rnd(1, 6, 2, 3), torch.randint(-1, 6, (1, 2, 3), generator=g)
+    mask = torch.rand(1, 6, 2, 3, generator=g) > 0.3
+    mask[0, :, 0, 0] = False
+    gl, ge, gs, gt = rnd(1, 2, 3), rnd(1, 2, 3), rnd(1, 2, 3), rnd(1, 2, 2, 3)
+    idx = torch.where(mask.gather(1, idx.clamp_min(0)[:, None])[:, 0], idx, torch.full_like(idx, -1))
+
+    def loss(v):
+        r = ref.stats(v, idx, 2, 2.0, mask)
+        fin = lambda t: torch.where(torch.isfinite(t), t, torch.zeros_like(t))
+        return (fin(r["log_prob"]) * gl + r["entropy"] * ge + fin(r["log_sum"]) * gs).sum() + (fin(r["top_log_prob"]) * gt).sum()
+
+    leaf = x.clone().requires_grad_(True)
+    auto, = torch.autograd.grad(loss(leaf), leaf)
+    want, _ = ref.gradient(x, idx, 2, 2.0, mask, gl, ge, gs, gt)
+    assert torch.allclose(want, torch.nan_to_num(auto), atol=1e-12)
+    eps = 1e-5
+    for k in range(x.numel()):
+        d = torch.zeros_like(x)
+        d.view(-1)[k] = eps
+        assert abs(float((loss(x + d) - loss(x - d)) / (2 * eps) - want.view(-1)[k])) < 1e-7

@@ -1,0 +1,423 @@
+"""plane_ops on the GPU against the 64-bit form in plane_ref (its error bounds are derived there)."""
+import math
+
+import pytest
+import torch
+
+import plane_ref as ref
+from doubletake_amd.modules import plane_ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+HALF_STEP = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+#: half the smallest step of the type: the rounding of values below its normal range
+TINY = {F32: 2.0 ** -150, F16: 2.0 ** -25, BF16: 2.0 ** -134}
+
+
+def make(shape, dtype=F32, layout="last", mask="none", seed=0, spread=3.0, ignore=0.2):
+    g = torch.Generator().manual_seed(seed)
+    b, D, h, w = shape
+    x = torch.randn(shape, generator=g) * spread
+    x[torch.rand(b, 1, h, w, generator=g).expand(shape) < 0.1] = 0.0   # equal scores
+    vol = x.to(dtype).to(DEV)
+    vol = vol.contiguous(memory_format=torch.channels_last) if layout == "last" else vol.contiguous()
+    m = None
+    if mask == "pixel":
+        m = torch.rand(b, 1, h, w, generator=g) > 0.2
+    elif mask == "plane":
+        m = (torch.rand(shape, generator=g) > 0.4) & (torch.rand(b, 1, h, w, generator=g) > 0.1)
+    elif mask == "batch":
+        m = torch.rand(1, D, 1, 1, generator=g) > 0.4
+    m = m.to(DEV) if m is not None else None
+    plane = torch.randint(0, D, (b, h, w), generator=g)
+    plane[torch.rand(b, h, w, generator=g) < ignore] = -1
+    plane[torch.rand(b, h, w, generator=g) < 0.05] = D
+    planes = torch.rand(b, D, 1, 1, generator=g).add(0.25).to(DEV)
+    return vol, m, plane.to(DEV), planes
+
+
+SHAPES = [(1, 1, 1, 1), (1, 2, 1, 3), (2, 3, 2, 2), (2, 7, 5, 9), (1, 8, 4, 4), (3, 16, 6, 11), (3, 33, 17, 19), (1, 64, 12, 20),
+          (2, 77, 6, 8), (1, 96, 16, 16), (2, 130, 6, 7), (1, 256, 9, 13), (1, 513, 5, 11), (1, 1500, 2, 3), (5, 4, 33, 31)]
+
+
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_stats(shape, dtype, layout):
+    for k, (mask, top, scale) in enumerate([("none", 0, 1.0), ("none", 8, 0.5), ("pixel", 1, 2.0), ("plane", 4, 1.0), ("plane", 8, 0.125),
+                                            ("batch", 3, 1.0), ("none", 2, 1.0)]):
+        top = min(top, shape[1])
+        vol, m, plane, planes = make(shape, dtype, layout, mask, seed=k)
+        planes = planes if top else None
+        keep = vol.clone()
+        res = plane_ops.plane_log_probs(vol, plane, top=top, scale=scale, mask_bdhw=m, depth_planes_bdhw=planes)
+        ref.check_stats(res, vol, plane, top, scale, m, planes)
+        assert torch.equal(vol, keep)
+        again = plane_ops.plane_log_probs(vol, plane.int(), top=top, scale=scale, mask_bdhw=m, depth_planes_bdhw=planes)
+        for a, b in zip(res, again):
+            assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_optional_inputs():
+    vol, m, plane, planes = make((2, 20, 5, 7))
+    r = plane_ops.plane_log_probs(vol)
+    ref.check_stats(r, vol)
+    assert r.top_depth_bkhw is None
+    r = plane_ops.plane_log_probs(vol, top=5)
+    ref.check_stats(r, vol, top=5)
+    # per-pixel planes, planes shared by the batch, planes of one pixel row
+    g = torch.Generator().manual_seed(1)
+    for shape in ((2, 20, 5, 7), (1, 20, 1, 1), (2, 20, 5, 1), (1, 20, 5, 7)):
+        pl = torch.rand(shape, generator=g).to(DEV)
+        r = plane_ops.plane_log_probs(vol, top=3, depth_planes_bdhw=pl)
+        ref.check_stats(r, vol, top=3, planes=pl)
+
+
+def test_empty_extents():
+    for shape in ((0, 4, 3, 3), (2, 4, 0, 3), (2, 4, 3, 0)):
+        vol = torch.zeros(shape, device=DEV, requires_grad=True)
+        b, _, h, w = shape
+        r = plane_ops.plane_log_probs(vol, torch.zeros(b, h, w, dtype=torch.int64, device=DEV), top=2)
+        assert r.log_prob_bhw.shape == (b, h, w) and r.top_plane_bkhw.shape == (b, 2, h, w)
+        grad, = torch.autograd.grad(r.entropy_bhw.sum(), vol)
+        assert grad.shape == shape
+        assert plane_ops.nearest_planes(torch.ones(b, h, w, device=DEV), torch.ones(1, 4, 1, 1, device=DEV)).shape == (b, h, w)
+
+
+def _views(dtype):
+    g = torch.Generator().manual_seed(5)
+    base = (torch.randn(3, 12, 10, 14, generator=g) * 2).to(dtype).to(DEV)
+    last = base.contiguous(memory_format=torch.channels_last)
+    flat = (torch.randn(1 + 2 * 9 * 5 * 7, generator=g)).to(dtype).to(DEV)
+    yield "crop first", base[:, :, 1:-2, 3:-1]
+    yield "crop last", last[:, :, 1:-2, 3:-1]
+    yield "plane slice first", base[:, 2:9]
+    yield "plane slice last", last[:, 2:9]
+    yield "plane step last", last[:, 1::3]
+    yield "pixel step", base[:, :, ::2, 1::3]
+    yield "pixel step last", last[:, :, ::2, 1::3]
+    yield "transposed", base.transpose(2, 3)
+    yield "planes on x", base.permute(0, 3, 1, 2)
+    yield "batch inside", base.permute(1, 0, 2, 3)
+    yield "one element off, first", flat[1:].view(2, 9, 5, 7)
+    yield "one element off, last", flat[1:].view(2, 5, 7, 9).permute(0, 3, 1, 2)
+    yield "broadcast batch", base[:1].expand(4, 12, 10, 14)
+    yield "broadcast pixels", base[:, :, :1, :1].expand(3, 12, 6, 5)
+    yield "broadcast planes", base[:, :1].expand(3, 7, 10, 14)
+    yield "rows of a wide map", base[:, :, :, :4]
+    yield "one pixel", last[:, :, 3:4, 5:6]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_views(dtype):
+    g = torch.Generator().manual_seed(6)
+    for name, v in _views(dtype):
+        b, D, h, w = v.shape
+        plane = torch.randint(-1, D, (b, h, w), generator=g).to(DEV)
+        mask = (torch.rand(b, h, D, w, generator=g) > 0.3).to(DEV).permute(0, 2, 1, 3)
+        try:
+            r = plane_ops.plane_log_probs(v, plane.transpose(1, 2).contiguous().transpose(1, 2), top=min(3, D), mask_bdhw=mask)
+            ref.check_stats(r, v, plane, min(3, D), 1.0, mask)
+            _check_grad(v, plane, min(2, D), 1.0, mask, seed=7)
+        except AssertionError as e:
+            raise AssertionError(f"{name}: {e}") from e
+
+
+def _check_grad(vol, plane, top, scale, mask, seed=0, use=("lp", "ent", "lsum", "top"), size=1.0):
+    g = torch.Generator().manual_seed(100 + seed)
+    b, D, h, w = vol.shape
+    leaf = vol.detach().requires_grad_(True)
+    r = plane_ops.plane_log_probs(leaf, plane, top=top, scale=scale, mask_bdhw=mask)
+    ref.check_stats(r, vol, plane, top, scale, mask)
+    gr = {"lp": (torch.randn(b, h, w, generator=g) * size).to(DEV) if plane is not None else None,
+          "ent": (torch.randn(b, h, w, generator=g) * size).to(DEV), "lsum": (torch.randn(b, h, w, generator=g) * size).to(DEV),
+          "top": (torch.randn(b, top, h, w, generator=g) * size).to(DEV) if top else None}
+    gr = {k: (v if k in use else None) for k, v in gr.items()}
+    pairs = [(o, gr[k]) for o, k in ((r.log_prob_bhw, "lp"), (r.entropy_bhw, "ent"), (r.log_sum_bhw, "lsum"), (r.top_log_prob_bkhw, "top"))
+             if gr[k] is not None]
+    grad, = torch.autograd.grad([o for o, _ in pairs], [leaf], [v for _, v in pairs])
+    want, err = ref.gradient(vol, plane, top, scale, mask, gr["lp"], gr["ent"], gr["lsum"], gr["top"])
+    assert grad.dtype == vol.dtype and grad.shape == vol.shape
+    ref.close(grad, want, err * (1 + HALF_STEP[vol.dtype]) + HALF_STEP[vol.dtype] * want.abs() + TINY[vol.dtype], 0.0, "gradient")
+    if mask is not None:
+        assert bool((grad[~mask.expand(vol.shape)] == 0).all())
+    return grad
+
+
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_gradient(shape, dtype, layout):
+    for k, (mask, top, scale, use) in enumerate([("none", 0, 1.0, ("lp",)), ("none", 2, 0.5, ("lp", "ent", "lsum", "top")),
+                                                 ("pixel", 8, 2.0, ("lp", "top")), ("plane", 4, 1.0, ("ent",)), ("plane", 1, 1.0, ("top", "lsum")),
+                                                 ("batch", 3, 0.125, ("lp", "ent"))]):
+        top = min(top, shape[1])
+        use = tuple(u for u in use if u != "top" or top)
+        vol, m, plane, _ = make(shape, dtype, layout, mask, seed=20 + k)
+        grad = _check_grad(vol, plane, top, scale, m, seed=k, use=use)
+        assert grad.stride() == torch.empty_like(vol).stride()
+
+
+def test_gradient_against_differences():
+    """(L(x + e) - L(x - e)) / 2e of the op's own outputs.  Truncation: e^2 / 6 times the third derivative, which for these losses is
+    below 64 (scale^3 (|g| + |g_ent| (|lp| + H) + ...) with factors below 4); rounding: two losses of at most 6 terms, each off by
+    bound_b + 4 u |value|, over 2e."""
+    g = torch.Generator().manual_seed(9)
+    vol = torch.randn(1, 6, 1, 2, generator=g).to(DEV)
+    plane = torch.tensor([[[2, 5]]], device=DEV)
+    eps = 2.0 ** -6
+
+    def loss(v):
+        r = plane_ops.plane_log_probs(v, plane, top=2)
+        return r.log_prob_bhw.double().sum() - 0.5 * r.entropy_bhw.double().sum() + 0.25 * r.top_log_prob_bkhw.double()[:, 1].sum()
+
+    leaf = vol.clone().requires_grad_(True)
+    grad, = torch.autograd.grad(loss(leaf), leaf)
+    tol = eps ** 2 / 6 * 64 + 2 * 6 * (ref.bound_b(6) + 4 * ref.U * 8) / (2 * eps)
+    for k in range(vol.numel()):
+        d = torch.zeros_like(vol)
+        d.view(-1)[k] = eps
+        num = float((loss(vol + d) - loss(vol - d)) / (2 * eps))
+        assert abs(num - float(grad.reshape(-1)[k])) < tol, k
+
+
+def test_gradient_of_broadcast_volume():
+    """Pixels that share one row of scores: the shared leaf gets the sum over the pixels."""
+    g = torch.Generator().manual_seed(10)
+    row = torch.randn(1, 9, 1, 1, generator=g).to(DEV)
+    plane = torch.randint(0, 9, (2, 4, 5), generator=g).to(DEV)
+    leaf = row.clone().requires_grad_(True)
+    r = plane_ops.plane_log_probs(leaf.expand(2, 9, 4, 5), plane)
+    r.log_prob_bhw.sum().backward()
+    full, err = ref.gradient(row.expand(2, 9, 4, 5), plane, 0, 1.0, None, torch.ones(2, 4, 5))
+    # 40 pixels summed by torch in float32: at most 40 roundings of partial sums below 40
+    ref.close(leaf.grad, full.sum((0, 2, 3), keepdim=True), (err + 2.0 ** -24 * full.abs()).sum((0, 2, 3), keepdim=True) + 40 * 40 * 2.0 ** -24)
+
+
+def test_gradient_of_several_calls_accumulates():
+    vol, m, plane, _ = make((2, 12, 6, 5), seed=40)
+    leaf = vol.clone().requires_grad_(True)
+    plane_ops.plane_log_probs(leaf, plane).log_prob_bhw.sum().backward()
+    one = leaf.grad.clone()
+    plane_ops.plane_log_probs(leaf, plane).log_prob_bhw.sum().backward()
+    assert torch.equal(leaf.grad, one + one)
+
+
+def test_no_gradient_where_none_is_asked_for():
+    vol, _, plane, planes = make((1, 9, 4, 5))
+    leaf = vol.requires_grad_(True)
+    with torch.no_grad():
+        assert not plane_ops.plane_log_probs(leaf, plane).log_prob_bhw.requires_grad
+    r = plane_ops.plane_log_probs(leaf, plane, top=2, depth_planes_bdhw=planes)
+    assert r.top_log_prob_bkhw.requires_grad and not r.top_plane_bkhw.requires_grad and not r.top_depth_bkhw.requires_grad
+    g1, = torch.autograd.grad(r.entropy_bhw.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g1.sum(), leaf)
+    r = plane_ops.plane_log_probs(leaf, plane)
+    with torch.no_grad():
+        leaf.add_(1.0)
+    with pytest.raises(RuntimeError):   # torch's own check: the saved volume was changed in place
+        r.entropy_bhw.sum().backward()
+
+
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [5, 64, 300])
+def test_edges(D, dtype, layout):
+    """One pixel per case: what masked places hold, rows without planes, lowest-value masks, infinities, NaN."""
+    low = torch.finfo(dtype).min
+    hi = torch.finfo(dtype).max
+    g = torch.Generator().manual_seed(D)
+    rows, masks = [], []
+
+    def add(fill, mask=None):
+        r = torch.randn(D, generator=g)
+        r = fill(r)
+        rows.append(r)
+        masks.append(torch.ones(D, dtype=torch.bool) if mask is None else mask)
+
+    def at(idx, v):
+        def f(r):
+            r[idx] = v
+            return r
+        return f
+
+    none = torch.zeros(D, dtype=torch.bool)
+    some = torch.rand(D, generator=g) > 0.5
+    some[0] = True
+    last = none.clone()
+    last[-1] = True
+    add(lambda r: r, none)                                   # nothing visible
+    add(at(slice(None), math.nan), none)                     # ... and NaN everywhere
+    add(at(slice(None), math.inf), none)
+    add(at(slice(None), -math.inf))                          # visible, without probability
+    add(at(slice(None), low))                                # a mask of the type's lowest value on all planes
+    add(at(slice(1, None), low))                             # ... on all but one
+    add(at(slice(0, D // 2), low))
+    add(at(slice(1, None), -math.inf))
+    add(lambda r: torch.where(some, r, torch.full_like(r, math.nan)), some)     # garbage behind the mask
+    add(lambda r: torch.where(some, r, torch.full_like(r, math.inf)), some)
+    add(lambda r: torch.where(some, r, torch.full_like(r, -math.inf)), some)
+    add(lambda r: r, last)                                   # one visible plane, the last
+    add(lambda r: r * 0)                                     # all equal
+    add(lambda r: torch.where(some, r * 0, -(r * 0)))        # +0 and -0 are equal
+    add(at(D // 2, math.nan))
+    add(at([0, D - 1], math.nan))
+    add(at(slice(None), math.nan))
+    add(at(1, math.inf))
+    add(at([1, D - 2], math.inf))
+    add(lambda r: at(0, math.nan)(at(2, math.inf)(r)))
+    add(at(3, hi))                                           # one plane far above the others
+    add(lambda r: at(3, hi)(at(2, low)(r)))
+    add(lambda r: r * 1e-8)
+    vol = torch.stack(rows, 1)[None, :, None, :].to(dtype).to(DEV)
+    mask = torch.stack(masks, 1)[None, :, None, :].to(DEV)
+    vol = vol.contiguous(memory_format=torch.channels_last) if layout == "last" else vol.contiguous()
+    n = vol.shape[-1]
+    for top, scale in ((0, 1.0), (5, 1.0), (3, 2.0), (5, 0.5)):
+        for pl in (0, 1, D - 1, -1, D):
+            plane = torch.full((1, 1, n), pl, device=DEV, dtype=torch.int64)
+            r = plane_ops.plane_log_probs(vol, plane, top=top, scale=scale, mask_bdhw=mask)
+            ref.check_stats(r, vol, plane, top, scale, mask)
+            leaf = vol.detach().requires_grad_(True)
+            r = plane_ops.plane_log_probs(leaf, plane, top=top, scale=scale, mask_bdhw=mask)
+            grad, = torch.autograd.grad([r.log_prob_bhw, r.entropy_bhw, r.log_sum_bhw],
+                                        [leaf], [torch.full_like(r.entropy_bhw, v) for v in (1.0, 0.5, -0.25)])
+            one = torch.ones(1, 1, n, dtype=torch.float64)
+            want, err = ref.gradient(vol, plane, top, scale, mask, one, 0.5 * one, -0.25 * one)
+            bad = torch.isnan(ref.stats(vol, None, 0, scale, mask)["entropy"])[0, 0]
+            assert int(bad.sum()) == 6
+            want[:, :, :, bad], err[:, :, :, bad] = 0.0, 0.0
+            grad = grad.cpu().clone()
+            assert bool((grad[~mask.cpu()] == 0).all())
+            assert bool(torch.isnan(grad[..., bad]).any(1).all())
+            grad[:, :, :, bad] = 0.0
+            ref.close(grad, want, err * (1 + HALF_STEP[dtype]) + HALF_STEP[dtype] * want.abs() + TINY[dtype], 0.0, f"gradient plane {pl}")
+
+
+def test_indices_beyond_32_bits():
+    """Offsets of the volume, of the mask, of the depth planes and of the gradient that pass 2^31 and 2^32 elements."""
+    far = (1 << 32) // 3 + 11
+    store = torch.zeros(4 * far + 64, dtype=F16, device=DEV)   # 11.5 GB
+    marks = torch.zeros(4 * far + 64, dtype=torch.bool, device=DEV)
+    g = torch.Generator().manual_seed(2)
+    vol = store.as_strided((1, 5, 4, 8), (0, far, 8, 1))
+    vol.copy_(torch.randn(1, 5, 4, 8, generator=g))
+    mask = marks.as_strided((1, 5, 4, 8), (0, far, 8, 1))
+    mask.copy_(torch.rand(1, 5, 4, 8, generator=g) > 0.3)
+    plane = torch.randint(-1, 5, (1, 4, 8), generator=g).to(DEV)
+    r = plane_ops.plane_log_probs(vol, plane, top=4, mask_bdhw=mask)
+    ref.check_stats(r, vol.contiguous(), plane, 4, 1.0, mask.contiguous())
+    del marks, mask
+    # planes next to each other, pixels far apart
+    vol = store.as_strided((1, 16, 1, 5), (0, 1, 0, far))
+    vol.copy_(torch.randn(1, 16, 1, 5, generator=g))
+    r = plane_ops.plane_log_probs(vol, top=4)
+    ref.check_stats(r, vol.contiguous(), top=4)
+    del store, vol
+    # a dense gradient of more than 2^32 bytes and 2^31 elements: the far end of a real volume
+    big = torch.empty(1, 16, 11586, 11586, dtype=F16, device=DEV).fill_(-1.0)
+    assert big.numel() > 1 << 31
+    tail = torch.randn(1, 16, 1, 40, generator=g).to(F16).to(DEV)
+    big[:, :, -1:, -40:] = tail
+    big.requires_grad_(True)
+    r = plane_ops.plane_log_probs(big, top=1)
+    cut = lambda t: t[..., -1:, -40:]
+    ref.close(cut(r.entropy_bhw), ref.stats(tail)["entropy"], ref.bound_b(16))
+    assert torch.equal(cut(r.top_plane_bkhw).cpu(), ref.stats(tail, top=1)["top_plane"])
+    assert torch.equal(r.entropy_bhw[0, 0, 0], r.entropy_bhw[0, -2, -2])
+    gs = torch.ones_like(r.log_sum_bhw)
+    grad, = torch.autograd.grad(r.log_sum_bhw, big, gs)
+    want, err = ref.gradient(tail, None, 0, 1.0, None, g_lsum=torch.ones(1, 1, 40))
+    ref.close(cut(grad), want, err * 1.01 + HALF_STEP[F16] * want.abs() + TINY[F16])
+    assert bool((grad[:, :, :-1] == 0.0625).all())
+
+
+@pytest.mark.parametrize("shape", [(1, 64, 12, 16), (2, 33, 7, 5)], ids=str)
+def test_side_stream_and_graph_replays(shape):
+    vol, m, plane, planes = make(shape, mask="plane", seed=50)
+    want = [t.clone() for t in plane_ops.plane_log_probs(vol, plane, top=3, mask_bdhw=m, depth_planes_bdhw=planes)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = plane_ops.plane_log_probs(vol, plane, top=3, mask_bdhw=m, depth_planes_bdhw=planes)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    static, dep = vol.clone(), torch.rand(shape[0], *shape[2:], device=DEV) + 0.25
+    gl = torch.ones_like(dep)
+
+    def step():
+        idx = plane_ops.nearest_planes(dep, planes)
+        leaf = static.detach().requires_grad_(True)
+        r = plane_ops.plane_log_probs(leaf, idx, top=3, mask_bdhw=m, depth_planes_bdhw=planes)
+        grad, = torch.autograd.grad([r.log_prob_bhw, r.entropy_bhw], [leaf], [gl, gl])
+        return [idx, grad] + [t.detach() for t in r]
+
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step()
+    for k in range(4):
+        static.copy_(make(shape, mask="plane", seed=60 + k)[0])
+        dep.copy_(torch.rand_like(dep) + 0.25)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), k
+
+
+def test_two_calls_at_once_on_two_streams():
+    cases = [make((2, 64, 30, 40), seed=70), make((1, 96, 60, 20), layout="first", seed=71)]
+    want = [plane_ops.plane_log_probs(v, p, top=4) for v, _, p, _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for st, (v, _, p, _) in zip(streams, cases):
+            with torch.cuda.stream(st):
+                got.append(plane_ops.plane_log_probs(v, p, top=4))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all((x is None and y is None) or torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_nearest_planes():
+    g = torch.Generator().manual_seed(11)
+    for b, D, h, w in ((1, 1, 1, 1), (2, 5, 3, 7), (1, 64, 12, 20), (3, 97, 5, 6), (1, 300, 2, 9)):
+        lin = 0.25 * (20.0 ** torch.linspace(0, 1, D))
+        for planes in (lin.view(1, D, 1, 1), lin.view(1, D, 1, 1) * (0.8 + 0.4 * torch.rand(b, 1, h, w, generator=g)),
+                       torch.rand(b, D, h, w, generator=g) * 5,                   # in no order
+                       torch.rand(b, D, 1, 1, generator=g).round(decimals=1) * 5 + 0.1,      # equal planes
+                       lin.flip(0).view(1, D, 1, 1).expand(b, D, 1, 1)):
+            dep = torch.rand(b, h, w, generator=g) * 7 - 0.5
+            flat = dep.view(-1)
+            for k, v in enumerate((math.nan, math.inf, -math.inf, -1.0, 0.0, 1e30, 1e-30)):
+                if k + 1 < flat.numel():
+                    flat[k + 1] = v
+            got = plane_ops.nearest_planes(dep.to(DEV), planes.to(DEV))
+            assert got.dtype == torch.int64 and torch.equal(got.cpu(), ref.nearest(dep, planes))
+    # half way between two planes: the lower one; planes themselves; NaN planes
+    planes = torch.tensor([1.0, 2.0, 4.0, math.nan, 8.0]).view(1, 5, 1, 1)
+    dep = torch.tensor([[[1.0, 1.5, 1.5000001, 3.0, 3.0000002, 6.0, 6.0000005, 8.0, 100.0]]])
+    got = plane_ops.nearest_planes(dep.to(DEV), planes.to(DEV))
+    assert got.cpu().tolist() == [[[0, 0, 1, 1, 2, 2, 4, 4, 4]]]
+    only_nan = torch.full((1, 3, 1, 1), math.nan)
+    assert plane_ops.nearest_planes(dep.to(DEV), only_nan.to(DEV)).cpu().tolist() == [[[-1] * 9]]
+    assert torch.equal(plane_ops.nearest_planes(dep.double().to(DEV), planes.to(DEV)).cpu(), ref.nearest(dep, planes))
+    wide = torch.rand(2, 6, 8, generator=g).to(DEV)
+    assert torch.equal(plane_ops.nearest_planes(wide[:, ::2, 1:-1], planes.to(DEV)).cpu(), ref.nearest(wide[:, ::2, 1:-1], planes))
+
+
+def test_depth_map_to_log_probability():
+    """The operators in a row, as the model uses them: a depth map's planes, their log probabilities, the alternatives' depths."""
+    vol, _, _, _ = make((2, 48, 9, 13), seed=80)
+    planes = (0.25 * 20.0 ** torch.linspace(0, 1, 48)).view(1, 48, 1, 1).to(DEV)
+    first = plane_ops.plane_log_probs(vol, top=1, depth_planes_bdhw=planes)
+    idx = plane_ops.nearest_planes(first.top_depth_bkhw[:, 0], planes)
+    assert torch.equal(idx, first.top_plane_bkhw[:, 0])
+    r = plane_ops.plane_log_probs(vol, idx, top=2, depth_planes_bdhw=planes)
+    assert torch.equal(r.log_prob_bhw, r.top_log_prob_bkhw[:, 0])
+    assert torch.equal(r.top_plane_bkhw[:, :1], first.top_plane_bkhw)
