@@ -6,8 +6,20 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
 #include <cmath>
+#include <cstdlib>
 
 namespace dt {
+
+// unsigned division by a launch constant (multiply, add, shift) for numerators below 2^31
+struct Div {
+  uint32_t mul, shift;
+};
+Div make_div(uint32_t d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return {(uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t n, Div d) { return (__umulhi(n, d.mul) + n) >> d.shift; }
 
 struct PlaneFwd {
   const void* vol;
@@ -20,6 +32,7 @@ struct PlaneFwd {
   int64_t vs[4], ms[4], ps[4];
   int b, d, h, w, top;
   float scale;
+  Div by_hw, by_w;
 };
 DT_ARG_POINTERS(PlaneFwd, offsetof(PlaneFwd, vol), offsetof(PlaneFwd, mask), offsetof(PlaneFwd, plane), offsetof(PlaneFwd, planes),
                 offsetof(PlaneFwd, log_prob), offsetof(PlaneFwd, entropy), offsetof(PlaneFwd, log_sum),
@@ -37,6 +50,7 @@ struct PlaneBwd {
   int64_t vs[4], ms[4], gs[4];
   int b, d, h, w, top;
   float scale;
+  Div by_hw, by_w;
 };
 DT_ARG_POINTERS(PlaneBwd, offsetof(PlaneBwd, vol), offsetof(PlaneBwd, mask), offsetof(PlaneBwd, plane), offsetof(PlaneBwd, entropy),
                 offsetof(PlaneBwd, top_plane), offsetof(PlaneBwd, row_max), offsetof(PlaneBwd, row_log),
@@ -49,6 +63,7 @@ struct PlaneNear {
   int64_t* out;
   int64_t ps[4];
   int b, d, h, w;
+  Div by_hw, by_w;
 };
 DT_ARG_POINTERS(PlaneNear, offsetof(PlaneNear, depth), offsetof(PlaneNear, planes), offsetof(PlaneNear, out));
 
@@ -65,14 +80,14 @@ template <>
 __device__ __forceinline__ __hip_bfloat16 from_f32<__hip_bfloat16>(float v) { return __float2bfloat16(v); }
 
 struct Pixel {
-  int b, y, x;
+  uint32_t b, y, x, r;  // r: index inside the image
 };
-__device__ __forceinline__ Pixel pixel_of(unsigned p, int h, int w) {
-  const unsigned row = p / (unsigned)w;
+__device__ __forceinline__ Pixel pixel_of(uint32_t p, int h, int w, Div by_hw, Div by_w) {
   Pixel q;
-  q.x = (int)(p - row * (unsigned)w);
-  q.b = (int)(row / (unsigned)h);
-  q.y = (int)(row - (unsigned)q.b * (unsigned)h);
+  q.b = divide(p, by_hw);
+  q.r = p - q.b * ((uint32_t)h * w);
+  q.y = divide(q.r, by_w);
+  q.x = q.r - q.y * w;
   return q;
 }
 __device__ __forceinline__ int64_t offset_of(const int64_t (&s)[4], const Pixel& q) { return q.b * s[0] + q.y * s[2] + q.x * s[3]; }
@@ -82,74 +97,289 @@ __device__ __forceinline__ float log_prob_of(float x, float m, float ls, float s
   return 2.f * ((0.5f * x - 0.5f * m) * scale) - ls;
 }
 
-// a before b among the alternatives: the larger score, NaN above everything, the lower plane of equals
-__device__ __forceinline__ bool ranks_above(float a, int ia, float b, int ib) {
-  const bool na = a != a, nb = b != b;
-  if (na != nb) return na;
-  if (!na && a != b) return a > b;
-  return (unsigned)ia < (unsigned)ib;  // (-1, an empty slot, ranks last)
+// ---- alternatives ------------------------------------------------------------------------------------------------------------
+// A score and its plane as ONE double, so that a compare-exchange of the ordered lists is one v_max_f64 and one v_min_f64: the
+// float's bits are the high word, which orders sign and magnitude like the float itself (its 8 exponent bits and 3 mantissa bits
+// become the double's 11 exponent bits; +-inf gives 0x7f8, so no score becomes a double NaN), and the plane is the low word,
+// complemented for positive scores: of equal scores the lower plane is the larger double.  -0 counts as +0; every NaN becomes
+// 0x7fe00000, above +inf.
+constexpr uint32_t kNone = 0xff800000u;  // -inf: a masked plane, an empty slot
+__device__ __forceinline__ double make_key(uint32_t hi, uint32_t lo) { return __longlong_as_double((long long)((uint64_t)hi << 32 | lo)); }
+__device__ __forceinline__ double key_of(float x, int plane) {
+  const float c = x + 0.f;
+  const uint32_t hi = c != c ? 0x7fe00000u : __float_as_uint(c);
+  return make_key(hi, (uint32_t)plane ^ ~(uint32_t)((int32_t)hi >> 31));
+}
+__device__ __forceinline__ uint32_t key_hi(double k) { return (uint32_t)((uint64_t)__double_as_longlong(k) >> 32); }
+__device__ __forceinline__ int key_plane(double k) {
+  return (int)((uint32_t)__double_as_longlong(k) ^ ~(uint32_t)((int32_t)key_hi(k) >> 31));
+}
+__device__ __forceinline__ void order(double& a, double& b) {
+  const double hi = fmax(a, b), lo = fmin(a, b);
+  a = hi, b = lo;
+}
+// descending sort of K keys (the smallest networks: 1, 5 and 19 exchanges)
+template <int K>
+__device__ __forceinline__ void sort_keys(double (&k)[K]) {
+  if constexpr (K == 4) {
+    order(k[0], k[2]), order(k[1], k[3]);
+    order(k[0], k[1]), order(k[2], k[3]);
+    order(k[1], k[2]);
+  } else if constexpr (K == 8) {
+    order(k[0], k[2]), order(k[1], k[3]), order(k[4], k[6]), order(k[5], k[7]);
+    order(k[0], k[4]), order(k[1], k[5]), order(k[2], k[6]), order(k[3], k[7]);
+    order(k[0], k[1]), order(k[2], k[3]), order(k[4], k[5]), order(k[6], k[7]);
+    order(k[2], k[4]), order(k[3], k[5]);
+    order(k[1], k[4]), order(k[3], k[6]);
+    order(k[1], k[2]), order(k[3], k[4]), order(k[5], k[6]);
+  }
+}
+// the K largest of two descending lists: the element-wise maxima of one against the other reversed are those K, and a bitonic
+// sequence, which log2 K rounds of exchanges put in order
+template <int K>
+__device__ __forceinline__ void merge_keys(double (&k)[K], const double (&o)[K]) {
+#pragma unroll
+  for (int i = 0; i < K; ++i) k[i] = fmax(k[i], o[K - 1 - i]);
+#pragma unroll
+  for (int dist = K / 2; dist > 0; dist /= 2)
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (!(i & dist)) order(k[i], k[i + dist]);
+}
+
+// ---- running statistics of one lane --------------------------------------------------------------------------------------------
+// m: largest score so far (-inf: none); s = sum exp(scale (x - m)); t = sum exp(y) y with y = scale (x - m).  When the maximum
+// moves by delta = scale (m_old - m_new): s' = s exp(delta), t' = (t + delta s) exp(delta).  A NaN score, or +inf (inf - inf), makes
+// s and with it every statistic NaN; the clamp keeps 0 * -inf out of t.
+constexpr float kLog2e = 1.4426950408889634f;
+template <int K>
+struct Stats {
+  float m = -INFINITY, s = 0.f, t = 0.f;
+  double key[K > 0 ? K : 1];
+  __device__ __forceinline__ Stats() {
+#pragma unroll
+    for (int j = 0; j < K; ++j) key[j] = make_key(kNone, 0xffffffffu);
+  }
+  __device__ __forceinline__ void rebase(float to, float scale) {
+    if (s != 0.f) {  // (nothing to move, and -inf - -inf, otherwise)
+      const float delta = fmaxf(scale * (m - to), -1e4f);
+      const float r = __builtin_amdgcn_exp2f(delta * kLog2e);
+      t = (t + delta * s) * r;
+      s *= r;
+    }
+    m = to;
+  }
+  // N more scores (masked ones are -inf); plane(e) numbers them in ascending order
+  template <int N, typename F>
+  __device__ __forceinline__ void add(const float (&x)[N], float scale, F plane) {
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
+    top = fmaxf(top, m);
+    if (top != m) rebase(top, scale);
+    const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float y = scale * (x[e] - m0);
+      const float ex = __builtin_amdgcn_exp2f(y * kLog2e);
+      s += ex;
+      t += ex * fmaxf(y, -1e4f);
+    }
+    if constexpr (K > 0) {
+      static_assert(N % K == 0);
+#pragma unroll
+      for (int c = 0; c < N; c += K) {
+        double k[K];
+#pragma unroll
+        for (int j = 0; j < K; ++j) k[j] = key_of(x[c + j], plane(c + j));
+        sort_keys(k);
+        merge_keys(key, k);
+      }
+    }
+  }
+  __device__ __forceinline__ void join(float om, float os, float ot, const double (&ok)[K > 0 ? K : 1], float scale) {
+    Stats o;
+    o.m = om, o.s = os, o.t = ot;
+    const float top = fmaxf(m, om);
+    if (top != m) rebase(top, scale);
+    if (top != om) o.rebase(top, scale);
+    s += o.s, t += o.t;
+    if constexpr (K > 0) merge_keys(key, ok);
+  }
+};
+
+// what a pixel's lane(s) write once its statistics are complete; lanes share the alternatives' slots (slot j belongs to lane j % lanes)
+template <int K>
+__device__ __forceinline__ void write_stats(const PlaneFwd& a, uint32_t p, const Pixel& q, const Stats<K>& st, int64_t given, float x_given,
+                                            int lane, int lanes) {
+  const float m = st.m == -INFINITY ? 0.f : st.m;
+  const bool empty = st.s == 0.f;
+  const float ls = logf(st.s);
+  if (lane == 0) {
+    a.entropy[p] = empty ? 0.f : ls - st.t / st.s;
+    a.log_sum[p] = m * a.scale + ls;
+    if (a.row_max) a.row_max[p] = m, a.row_log[p] = ls;
+    if (a.plane) a.log_prob[p] = given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale);
+  }
+  if constexpr (K > 0) {
+    const size_t hw = (size_t)a.h * a.w;
+    const size_t o = (size_t)q.b * a.top * hw + q.r;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (j >= a.top) break;
+      if (lane != j % lanes) continue;
+      const bool none = key_hi(st.key[j]) == kNone;
+      const int at = key_plane(st.key[j]);
+      a.top_plane[o + j * hw] = none ? -1 : at;
+      a.top_log_prob[o + j * hw] = none ? -INFINITY : log_prob_of(__uint_as_float(key_hi(st.key[j])), m, ls, a.scale);
+      if (a.top_depth) a.top_depth[o + j * hw] = none ? 0.f : a.planes[offset_of(a.ps, q) + at * a.ps[1]];
+    }
+  }
+}
+
+// the score of one plane of a pixel, -inf where the mask hides it
+template <typename T>
+__device__ __forceinline__ float score_at(const T* vol, const uint8_t* mask, int64_t vs, int64_t ms, int d) {
+  return mask && !mask[d * ms] ? -INFINITY : to_f32(vol[d * vs]);
+}
+
+// Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel, 16 planes at a time in registers.
+// S waves of the workgroup share 64 pixels, each takes a contiguous range of planes, and the first joins the S partial results.
+template <typename T, int K, int S>
+__global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
+  constexpr int kPixels = 256 / S, kN = 16;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const uint32_t p = blockIdx.x * kPixels + (S == 1 ? threadIdx.x : lane);
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  const bool live = p < pixels;
+  const Pixel q = pixel_of(live ? p : pixels - 1, a.h, a.w, a.by_hw, a.by_w);
+  const T* vol = (const T*)a.vol + offset_of(a.vs, q);
+  const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
+  int64_t given = -1;
+  float x_given = 0.f;
+  if (a.plane && (S == 1 || wave == 0)) {
+    given = a.plane[live ? p : pixels - 1];
+    if (given >= 0 && given < a.d) x_given = score_at(vol, mask, a.vs[1], a.ms[1], (int)given);
+  }
+  const int part = S == 1 ? a.d : (a.d + S - 1) / S;
+  const int begin = S == 1 ? 0 : wave * part, end = min(a.d, begin + part);
+  Stats<K> st;
+  for (int d0 = begin; d0 < end; d0 += kN) {
+    float x[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) x[e] = d0 + e < end ? to_f32(vol[(d0 + e) * a.vs[1]]) : -INFINITY;
+    if (mask) {
+      uint8_t seen[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) seen[e] = d0 + e < end ? mask[(d0 + e) * a.ms[1]] : 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? x[e] : -INFINITY;
+    }
+    st.add(x, a.scale, [&](int e) { return d0 + e; });
+  }
+  if constexpr (S > 1) {
+    __shared__ float part_f[S - 1][3][64];
+    __shared__ double part_k[S - 1][K > 0 ? K : 1][64];
+    if (wave > 0) {
+      part_f[wave - 1][0][lane] = st.m, part_f[wave - 1][1][lane] = st.s, part_f[wave - 1][2][lane] = st.t;
+#pragma unroll
+      for (int j = 0; j < K; ++j) part_k[wave - 1][j][lane] = st.key[j];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int o = 0; o < S - 1; ++o) {
+      double k[K > 0 ? K : 1];
+#pragma unroll
+      for (int j = 0; j < K; ++j) k[j] = part_k[o][j][lane];
+      st.join(part_f[o][0][lane], part_f[o][1][lane], part_f[o][2][lane], k, a.scale);
+    }
+  }
+  if (live) write_stats<K>(a, p, q, st, given, x_given, 0, 1);
+}
+
+// exchange with the lane of another group of 1, 2, 4 or 8 lanes of the same row of 16 (the groups' lanes hold equal values)
+template <int STEP>
+__device__ __forceinline__ uint32_t other_u32(uint32_t v) {
+  constexpr int ctrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;  // quad_perm 1,0,3,2 / 2,3,0,1; half mirror; mirror
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);
+}
+template <int STEP>
+__device__ __forceinline__ float other(float v) { return __uint_as_float(other_u32<STEP>(__float_as_uint(v))); }
+template <int STEP>
+__device__ __forceinline__ double other(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  return make_key(other_u32<STEP>((uint32_t)(b >> 32)), other_u32<STEP>((uint32_t)b));
+}
+template <int K, int STEP>
+__device__ __forceinline__ void join_lanes(Stats<K>& st, float scale) {
+  double k[K > 0 ? K : 1];
+#pragma unroll
+  for (int j = 0; j < K; ++j) k[j] = other<STEP>(st.key[j]);
+  st.join(other<STEP>(st.m), other<STEP>(st.s), other<STEP>(st.t), k, scale);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) plane_stats_kernel(PlaneFwd a) {
-  const unsigned p = blockIdx.x * 256u + threadIdx.x;
-  if (p >= (unsigned)a.b * a.h * a.w) return;
-  const Pixel q = pixel_of(p, a.h, a.w);
+struct Vec16 {  // 16 bytes of scores, aligned like one score: global loads need no more
+  static constexpr int n = 16 / sizeof(T);
+  T v[n];
+};
+
+// Volume with the planes of a pixel next to each other (channels_last): G lanes per pixel, 16 bytes of scores per lane and load.
+template <typename T, int K, int G>
+__global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
+  constexpr int kN = 16, kVec = Vec16<T>::n, kStep = G * kVec;
+  const int lane = threadIdx.x % G;
+  const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  const bool live = p < pixels;
+  const Pixel q = pixel_of(live ? p : pixels - 1, a.h, a.w, a.by_hw, a.by_w);
   const T* vol = (const T*)a.vol + offset_of(a.vs, q);
   const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
-  auto score = [&](int d) { return mask && !mask[d * a.ms[1]] ? -INFINITY : to_f32(vol[d * a.vs[1]]); };
-  float m = -INFINITY;
-  float tv[DT_PLANE_MAX_TOP];
-  int ti[DT_PLANE_MAX_TOP];
-#pragma unroll
-  for (int j = 0; j < DT_PLANE_MAX_TOP; ++j) tv[j] = -INFINITY, ti[j] = -1;
-  for (int d = 0; d < a.d; ++d) {
-    float x = score(d);
-    m = fmaxf(m, x);
-    if (x == -INFINITY) continue;
-    int i = d;
-#pragma unroll
-    for (int j = 0; j < DT_PLANE_MAX_TOP; ++j) {
-      const bool take = ti[j] < 0 || ranks_above(x, i, tv[j], ti[j]);
-      const float xv = tv[j];
-      const int xi = ti[j];
-      tv[j] = take ? x : xv, ti[j] = take ? i : xi;
-      x = take ? xv : x, i = take ? xi : i;
-    }
-  }
-  const float m0 = m == -INFINITY ? 0.f : m;
-  float s = 0.f, t = 0.f;
-  for (int d = 0; d < a.d; ++d) {
-    const float y = a.scale * (score(d) - m0);
-    const float e = expf(y);
-    s += e;
-    t += e * fmaxf(y, -1e4f);
-  }
-  const bool empty = s == 0.f;
-  const float ls = logf(s);
-  a.entropy[p] = empty ? 0.f : ls - t / s;
-  a.log_sum[p] = m0 * a.scale + ls;
-  if (a.row_max) a.row_max[p] = m0, a.row_log[p] = ls;
+  int64_t given = -1;
+  float x_given = 0.f;
   if (a.plane) {
-    const int64_t g = a.plane[p];
-    a.log_prob[p] = g < 0 || g >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(score((int)g), m0, ls, a.scale);
+    given = a.plane[live ? p : pixels - 1];
+    if (given >= 0 && given < a.d) x_given = score_at(vol, mask, 1, a.ms[1], (int)given);
   }
-  const size_t hw = (size_t)a.h * a.w;
-  const size_t o = (size_t)q.b * a.top * hw + (size_t)q.y * a.w + q.x;
+  Stats<K> st;
+  for (int d0 = 0; d0 < a.d; d0 += kN * G) {
+    float x[kN];
+    auto plane = [&](int e) { return d0 + (e / kVec) * kStep + lane * kVec + e % kVec; };
 #pragma unroll
-  for (int j = 0; j < DT_PLANE_MAX_TOP; ++j) {
-    if (j >= a.top) break;
-    a.top_plane[o + j * hw] = ti[j];
-    a.top_log_prob[o + j * hw] = ti[j] < 0 ? -INFINITY : log_prob_of(tv[j], m0, ls, a.scale);
-    if (a.top_depth) a.top_depth[o + j * hw] = ti[j] < 0 ? 0.f : a.planes[offset_of(a.ps, q) + ti[j] * a.ps[1]];
+    for (int e = 0; e < kN; e += kVec) {
+      const int d = plane(e);
+      if (d + kVec <= a.d) {
+        Vec16<T> v;
+        __builtin_memcpy(&v, vol + d, sizeof v);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[e + j] = to_f32(v.v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[e + j] = d + j < a.d ? to_f32(vol[d + j]) : -INFINITY;
+      }
+    }
+    if (mask) {
+      uint8_t seen[kN];
+#pragma unroll
+      for (int e = 0; e < kN; ++e) seen[e] = plane(e) < a.d ? mask[plane(e) * a.ms[1]] : 0;
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? x[e] : -INFINITY;
+    }
+    st.add(x, a.scale, plane);
   }
+  if constexpr (G >= 2) join_lanes<K, 1>(st, a.scale);
+  if constexpr (G >= 4) join_lanes<K, 2>(st, a.scale);
+  if constexpr (G >= 8) join_lanes<K, 4>(st, a.scale);
+  if constexpr (G >= 16) join_lanes<K, 8>(st, a.scale);
+  if (live) write_stats<K>(a, p, q, st, given, x_given, lane, G);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) plane_grad_kernel(PlaneBwd a) {
   const unsigned p = blockIdx.x * 256u + threadIdx.x;
   if (p >= (unsigned)a.b * a.h * a.w) return;
-  const Pixel q = pixel_of(p, a.h, a.w);
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const T* vol = (const T*)a.vol + offset_of(a.vs, q);
   T* grad = (T*)a.grad + offset_of(a.gs, q);
   const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
@@ -166,7 +396,7 @@ __global__ void __launch_bounds__(256) plane_grad_kernel(PlaneBwd a) {
   int ti[DT_PLANE_MAX_TOP];
   float tg[DT_PLANE_MAX_TOP];
   const size_t hw = (size_t)a.h * a.w;
-  const size_t o = (size_t)q.b * a.top * hw + (size_t)q.y * a.w + q.x;
+  const size_t o = (size_t)q.b * a.top * hw + q.r;
 #pragma unroll
   for (int j = 0; j < DT_PLANE_MAX_TOP; ++j) {
     ti[j] = -1, tg[j] = 0.f;
@@ -194,7 +424,7 @@ __global__ void __launch_bounds__(256) plane_grad_kernel(PlaneBwd a) {
 __global__ void __launch_bounds__(256) nearest_planes_kernel(PlaneNear a) {
   const unsigned p = blockIdx.x * 256u + threadIdx.x;
   if (p >= (unsigned)a.b * a.h * a.w) return;
-  const Pixel q = pixel_of(p, a.h, a.w);
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const float* planes = a.planes + offset_of(a.ps, q);
   const float depth = a.depth[p];
   int at = -1;
@@ -209,11 +439,32 @@ __global__ void __launch_bounds__(256) nearest_planes_kernel(PlaneNear a) {
 }
 
 template <typename F>
-int by_type(int dtype, F&& f) {
-  switch (dtype) {
-    case DT_VOL_F32: return f(float{});
-    case DT_VOL_F16: return f(__half{});
-    default: return f(__hip_bfloat16{});
+void by_type(int dtype, F&& f) {
+  if (dtype == DT_VOL_F32) f(float{});
+  else if (dtype == DT_VOL_F16) f(__half{});
+  else f(__hip_bfloat16{});
+}
+
+// lists of 0, 1, 4 and 8 slots
+template <typename F>
+void by_top(int top, F&& f) {
+  if (top == 0) f(std::integral_constant<int, 0>{});
+  else if (top == 1) f(std::integral_constant<int, 1>{});
+  else if (top <= 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 8>{});
+}
+
+template <typename T, int K>
+void launch_stats(const PlaneFwd& a, hipStream_t s) {
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  static const int force = getenv("DT_PLANE_VAR") ? atoi(getenv("DT_PLANE_VAR")) : 0;  // EXPERIMENT
+  if (a.vs[1] == 1) {
+    if (force == 16) DT_LAUNCH((plane_stats_last_kernel<T, K, 16>), dim3((pixels + 15) / 16), dim3(256), 0, s, a);
+    else if (force == 8) DT_LAUNCH((plane_stats_last_kernel<T, K, 8>), dim3((pixels + 31) / 32), dim3(256), 0, s, a);
+    else DT_LAUNCH((plane_stats_last_kernel<T, K, 4>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
+  } else {
+    if (force == 1) DT_LAUNCH((plane_stats_first_kernel<T, K, 1>), dim3((pixels + 255) / 256), dim3(256), 0, s, a);
+    else DT_LAUNCH((plane_stats_first_kernel<T, K, 4>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
   }
 }
 
@@ -246,11 +497,11 @@ int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint
   PlaneFwd a{volume, mask, plane_bhw, depth_planes, log_prob, entropy, log_sum, top_log_prob, top_plane, top_depth, row_max, row_log};
   for (int i = 0; i < 4; ++i) a.vs[i] = d->vol_stride[i], a.ms[i] = d->mask_stride[i], a.ps[i] = d->planes_stride[i];
   a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
-  const unsigned pixels = (unsigned)d->b * d->h * d->w;
-  return by_type(d->dtype, [&](auto v) {
-    DT_LAUNCH(plane_stats_kernel<decltype(v)>, dim3((pixels + 255) / 256), dim3(256), 0, to_stream(s), a);
-    return check_launch("dt_cv_plane_log_probs");
+  a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
+  by_type(d->dtype, [&](auto v) {
+    by_top(d->top, [&](auto k) { launch_stats<decltype(v), k.value>(a, to_stream(s)); });
   });
+  return check_launch("dt_cv_plane_log_probs");
 }
 
 int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const uint8_t* mask, const int64_t* plane_bhw,
@@ -264,11 +515,12 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
   PlaneBwd a{volume, mask, plane_bhw, entropy, top_plane, row_max, row_log, g_log_prob, g_entropy, g_log_sum, g_top_log_prob, grad_volume};
   for (int i = 0; i < 4; ++i) a.vs[i] = d->vol_stride[i], a.ms[i] = d->mask_stride[i], a.gs[i] = d->grad_stride[i];
   a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
+  a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
   const unsigned pixels = (unsigned)d->b * d->h * d->w;
-  return by_type(d->dtype, [&](auto v) {
+  by_type(d->dtype, [&](auto v) {
     DT_LAUNCH(plane_grad_kernel<decltype(v)>, dim3((pixels + 255) / 256), dim3(256), 0, to_stream(s), a);
-    return check_launch("dt_cv_plane_log_probs_grad");
   });
+  return check_launch("dt_cv_plane_log_probs_grad");
 }
 
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
@@ -279,6 +531,7 @@ int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, 
   PlaneNear a{depth_bhw, depth_planes, plane_bhw};
   for (int i = 0; i < 4; ++i) a.ps[i] = planes_stride4[i];
   a.b = b, a.d = d, a.h = h, a.w = w;
+  a.by_hw = make_div((uint32_t)h * w), a.by_w = make_div(w);
   const unsigned pixels = (unsigned)b * h * w;
   DT_LAUNCH(nearest_planes_kernel, dim3((pixels + 255) / 256), dim3(256), 0, to_stream(s), a);
   return check_launch("dt_cv_nearest_planes_f32");
