@@ -5,6 +5,7 @@
 
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
+#include <algorithm>
 #include <cmath>
 #include <cstdlib>
 
@@ -148,10 +149,10 @@ __device__ __forceinline__ void merge_keys(double (&k)[K], const double (&o)[K])
 }
 
 // ---- running statistics of one lane --------------------------------------------------------------------------------------------
-// m: largest score so far (-inf: none); s = sum exp(scale (x - m)); t = sum exp(y) y with y = scale (x - m).  When the maximum
-// moves by delta = scale (m_old - m_new): s' = s exp(delta), t' = (t + delta s) exp(delta).  A NaN score, or +inf (inf - inf), makes
-// s and with it every statistic NaN; the clamp keeps 0 * -inf out of t.
-constexpr float kLog2e = 1.4426950408889634f;
+// m: largest score so far (-inf: none); with y = c (x - m), c = scale log2 e: s = sum 2^y and t = sum 2^y y.  When the maximum moves
+// by delta = c (m_old - m_new): s' = s 2^delta, t' = (t + delta s) 2^delta.  A NaN score, or +inf (inf - inf), makes s and with it
+// every statistic NaN; the clamp keeps 0 * -inf out of t.  Differences come before the product: scores far from zero lose nothing.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int K>
 struct Stats {
   float m = -INFINITY, s = 0.f, t = 0.f;
@@ -160,10 +161,10 @@ struct Stats {
 #pragma unroll
     for (int j = 0; j < K; ++j) key[j] = make_key(kNone, 0xffffffffu);
   }
-  __device__ __forceinline__ void rebase(float to, float scale) {
+  __device__ __forceinline__ void rebase(float to, float c) {
     if (s != 0.f) {  // (nothing to move, and -inf - -inf, otherwise)
-      const float delta = fmaxf(scale * (m - to), -1e4f);
-      const float r = __builtin_amdgcn_exp2f(delta * kLog2e);
+      const float delta = fmaxf(c * (m - to), -1e4f);
+      const float r = __builtin_amdgcn_exp2f(delta);
       t = (t + delta * s) * r;
       s *= r;
     }
@@ -171,38 +172,37 @@ struct Stats {
   }
   // N more scores (masked ones are -inf); plane(e) numbers them in ascending order
   template <int N, typename F>
-  __device__ __forceinline__ void add(const float (&x)[N], float scale, F plane) {
-    float top = x[0];
+  __device__ __forceinline__ void add(const float (&x)[N], float c, F plane) {
+    float top = m;
 #pragma unroll
-    for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-    top = fmaxf(top, m);
-    if (top != m) rebase(top, scale);
+    for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
+    if (top != m) rebase(top, c);
     const float m0 = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float y = scale * (x[e] - m0);
-      const float ex = __builtin_amdgcn_exp2f(y * kLog2e);
+      const float y = c * (x[e] - m0);
+      const float ex = __builtin_amdgcn_exp2f(y);
       s += ex;
       t += ex * fmaxf(y, -1e4f);
     }
     if constexpr (K > 0) {
       static_assert(N % K == 0);
 #pragma unroll
-      for (int c = 0; c < N; c += K) {
+      for (int b = 0; b < N; b += K) {
         double k[K];
 #pragma unroll
-        for (int j = 0; j < K; ++j) k[j] = key_of(x[c + j], plane(c + j));
+        for (int j = 0; j < K; ++j) k[j] = key_of(x[b + j], plane(b + j));
         sort_keys(k);
         merge_keys(key, k);
       }
     }
   }
-  __device__ __forceinline__ void join(float om, float os, float ot, const double (&ok)[K > 0 ? K : 1], float scale) {
+  __device__ __forceinline__ void join(float om, float os, float ot, const double (&ok)[K > 0 ? K : 1], float c) {
     Stats o;
     o.m = om, o.s = os, o.t = ot;
     const float top = fmaxf(m, om);
-    if (top != m) rebase(top, scale);
-    if (top != om) o.rebase(top, scale);
+    if (top != m) rebase(top, c);
+    if (top != om) o.rebase(top, c);
     s += o.s, t += o.t;
     if constexpr (K > 0) merge_keys(key, ok);
   }
@@ -216,7 +216,7 @@ __device__ __forceinline__ void write_stats(const PlaneFwd& a, uint32_t p, const
   const bool empty = st.s == 0.f;
   const float ls = logf(st.s);
   if (lane == 0) {
-    a.entropy[p] = empty ? 0.f : ls - st.t / st.s;
+    a.entropy[p] = empty ? 0.f : ls - kLn2 * (st.t / st.s);
     a.log_sum[p] = m * a.scale + ls;
     if (a.row_max) a.row_max[p] = m, a.row_log[p] = ls;
     if (a.plane) a.log_prob[p] = given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale);
@@ -237,45 +237,61 @@ __device__ __forceinline__ void write_stats(const PlaneFwd& a, uint32_t p, const
   }
 }
 
+// Scores are addressed as a launch-uniform 64-bit base (scalar registers) plus an offset per lane of type Off: 32 bits where every
+// pixel lies within 4 GB of the first, which costs no vector arithmetic per load, 64 bits otherwise.
+template <typename T, typename Off>
+__device__ __forceinline__ T load(const void* base, Off off) { return *(const T*)((const char*)base + off); }
+
 // the score of one plane of a pixel, -inf where the mask hides it
-template <typename T>
-__device__ __forceinline__ float score_at(const T* vol, const uint8_t* mask, int64_t vs, int64_t ms, int d) {
-  return mask && !mask[d * ms] ? -INFINITY : to_f32(vol[d * vs]);
+template <typename T, typename Off>
+__device__ __forceinline__ float score_at(const PlaneFwd& a, Off vo, Off mo, int64_t d) {
+  const bool seen = !a.mask || a.mask[d * a.ms[1] + mo];
+  return seen ? to_f32(*(const T*)((const char*)a.vol + d * a.vs[1] * (int64_t)sizeof(T) + vo)) : -INFINITY;
 }
 
-// Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel, 16 planes at a time in registers.
+// Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel, 16 planes at a time in registers,
+// all their loads in flight together (planes past the end read the last one again and count as -inf).
 // S waves of the workgroup share 64 pixels, each takes a contiguous range of planes, and the first joins the S partial results.
-template <typename T, int K, int S>
+template <typename T, int K, int S, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   constexpr int kPixels = 256 / S, kN = 16;
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const uint32_t p = blockIdx.x * kPixels + (S == 1 ? threadIdx.x : lane);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+  const uint32_t at = blockIdx.x * kPixels + (S == 1 ? threadIdx.x : lane);
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  const bool live = p < pixels;
-  const Pixel q = pixel_of(live ? p : pixels - 1, a.h, a.w, a.by_hw, a.by_w);
-  const T* vol = (const T*)a.vol + offset_of(a.vs, q);
-  const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
+  const bool live = at < pixels;
+  const uint32_t p = live ? at : pixels - 1;
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
+  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q);
+  const float c = a.scale * kLog2e;
   int64_t given = -1;
   float x_given = 0.f;
   if (a.plane && (S == 1 || wave == 0)) {
-    given = a.plane[live ? p : pixels - 1];
-    if (given >= 0 && given < a.d) x_given = score_at(vol, mask, a.vs[1], a.ms[1], (int)given);
+    given = a.plane[p];
+    if (given >= 0 && given < a.d) x_given = score_at<T>(a, vo, mo, given);
   }
   const int part = S == 1 ? a.d : (a.d + S - 1) / S;
   const int begin = S == 1 ? 0 : wave * part, end = min(a.d, begin + part);
   Stats<K> st;
   for (int d0 = begin; d0 < end; d0 += kN) {
-    float x[kN];
+    T raw[kN];
 #pragma unroll
-    for (int e = 0; e < kN; ++e) x[e] = d0 + e < end ? to_f32(vol[(d0 + e) * a.vs[1]]) : -INFINITY;
-    if (mask) {
+    for (int e = 0; e < kN; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, end - 1) * a.vs[1], vo);
+    float x[kN];
+    if (a.mask) {
       uint8_t seen[kN];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) seen[e] = d0 + e < end ? mask[(d0 + e) * a.ms[1]] : 0;
+      for (int e = 0; e < kN; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, end - 1) * a.ms[1], mo);
 #pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? x[e] : -INFINITY;
+      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
     }
-    st.add(x, a.scale, [&](int e) { return d0 + e; });
+    if (d0 + kN > end) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = d0 + e < end ? x[e] : -INFINITY;
+    }
+    st.add(x, c, [&](int e) { return d0 + e; });
   }
   if constexpr (S > 1) {
     __shared__ float part_f[S - 1][3][64];
@@ -292,7 +308,7 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
       double k[K > 0 ? K : 1];
 #pragma unroll
       for (int j = 0; j < K; ++j) k[j] = part_k[o][j][lane];
-      st.join(part_f[o][0][lane], part_f[o][1][lane], part_f[o][2][lane], k, a.scale);
+      st.join(part_f[o][0][lane], part_f[o][1][lane], part_f[o][2][lane], k, c);
     }
   }
   if (live) write_stats<K>(a, p, q, st, given, x_given, 0, 1);
@@ -312,11 +328,11 @@ __device__ __forceinline__ double other(double v) {
   return make_key(other_u32<STEP>((uint32_t)(b >> 32)), other_u32<STEP>((uint32_t)b));
 }
 template <int K, int STEP>
-__device__ __forceinline__ void join_lanes(Stats<K>& st, float scale) {
+__device__ __forceinline__ void join_lanes(Stats<K>& st, float c) {
   double k[K > 0 ? K : 1];
 #pragma unroll
   for (int j = 0; j < K; ++j) k[j] = other<STEP>(st.key[j]);
-  st.join(other<STEP>(st.m), other<STEP>(st.s), other<STEP>(st.t), k, scale);
+  st.join(other<STEP>(st.m), other<STEP>(st.s), other<STEP>(st.t), k, c);
 }
 
 template <typename T>
@@ -326,116 +342,201 @@ struct Vec16 {  // 16 bytes of scores, aligned like one score: global loads need
 };
 
 // Volume with the planes of a pixel next to each other (channels_last): G lanes per pixel, 16 bytes of scores per lane and load.
-template <typename T, int K, int G>
+template <typename T, int K, int G, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   constexpr int kN = 16, kVec = Vec16<T>::n, kStep = G * kVec;
   const int lane = threadIdx.x % G;
-  const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
+  const uint32_t at = blockIdx.x * (256u / G) + threadIdx.x / G;
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  const bool live = p < pixels;
-  const Pixel q = pixel_of(live ? p : pixels - 1, a.h, a.w, a.by_hw, a.by_w);
-  const T* vol = (const T*)a.vol + offset_of(a.vs, q);
-  const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
+  const bool live = at < pixels;
+  const uint32_t p = live ? at : pixels - 1;
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
+  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q);
+  const float c = a.scale * kLog2e;
   int64_t given = -1;
   float x_given = 0.f;
   if (a.plane) {
-    given = a.plane[live ? p : pixels - 1];
-    if (given >= 0 && given < a.d) x_given = score_at(vol, mask, 1, a.ms[1], (int)given);
+    given = a.plane[p];
+    if (given >= 0 && given < a.d) x_given = score_at<T>(a, vo, mo, given);
   }
   Stats<K> st;
   for (int d0 = 0; d0 < a.d; d0 += kN * G) {
-    float x[kN];
+    const bool whole = d0 + kN * G <= a.d;
+    T raw[kN];
     auto plane = [&](int e) { return d0 + (e / kVec) * kStep + lane * kVec + e % kVec; };
 #pragma unroll
     for (int e = 0; e < kN; e += kVec) {
       const int d = plane(e);
-      if (d + kVec <= a.d) {
-        Vec16<T> v;
-        __builtin_memcpy(&v, vol + d, sizeof v);
+      if (whole || d + kVec <= a.d) {
+        const Vec16<T> v = load<Vec16<T>>((const T*)a.vol + d0 + (e / kVec) * kStep, (Off)(vo + lane * 16u));
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[e + j] = to_f32(v.v[j]);
+        for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
       } else {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[e + j] = d + j < a.d ? to_f32(vol[d + j]) : -INFINITY;
+        for (int j = 0; j < kVec; ++j) raw[e + j] = load<T>((const T*)a.vol, (Off)(vo + min(d + j, a.d - 1) * sizeof(T)));
       }
     }
-    if (mask) {
+    float x[kN];
+    if (a.mask) {
       uint8_t seen[kN];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) seen[e] = plane(e) < a.d ? mask[plane(e) * a.ms[1]] : 0;
+      for (int e = 0; e < kN; ++e) seen[e] = a.mask[min(plane(e), a.d - 1) * a.ms[1] + mo];
 #pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? x[e] : -INFINITY;
+      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
     }
-    st.add(x, a.scale, plane);
+    if (!whole) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = plane(e) < a.d ? x[e] : -INFINITY;
+    }
+    st.add(x, c, plane);
   }
-  if constexpr (G >= 2) join_lanes<K, 1>(st, a.scale);
-  if constexpr (G >= 4) join_lanes<K, 2>(st, a.scale);
-  if constexpr (G >= 8) join_lanes<K, 4>(st, a.scale);
-  if constexpr (G >= 16) join_lanes<K, 8>(st, a.scale);
+  if constexpr (G >= 2) join_lanes<K, 1>(st, c);
+  if constexpr (G >= 4) join_lanes<K, 2>(st, c);
+  if constexpr (G >= 8) join_lanes<K, 4>(st, c);
+  if constexpr (G >= 16) join_lanes<K, 8>(st, c);
   if (live) write_stats<K>(a, p, q, st, given, x_given, lane, G);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) plane_grad_kernel(PlaneBwd a) {
-  const unsigned p = blockIdx.x * 256u + threadIdx.x;
-  if (p >= (unsigned)a.b * a.h * a.w) return;
+// ---- gradient ------------------------------------------------------------------------------------------------------------------
+// What a pixel contributes to each of its planes: with l = c (x - m) - log2 s the plane's log probability in base 2,
+//   dx = 2^l (k0 + k1 max(l, -1e4)) + (gradient of the slot that names the plane),
+//   k0 = scale (g_log_sum - g_log_prob - sum g_top - g_entropy entropy), k1 = -scale g_entropy ln 2.
+// Slots: the alternatives and the given plane, which is folded into the alternative it coincides with; all planes differ.
+template <int K>
+struct Pull {
+  float m, ls2, c, k0, k1;
+  int at[K + 1];
+  float g[K + 1];
+  __device__ __forceinline__ Pull(const PlaneBwd& a, uint32_t p, const Pixel& q) {
+    m = a.row_max[p], ls2 = a.row_log[p] * kLog2e, c = a.scale * kLog2e;
+    const float ge = a.g_entropy ? a.g_entropy[p] : 0.f;
+    float all = a.g_log_sum ? a.g_log_sum[p] : 0.f;
+    at[K] = -1, g[K] = 0.f;
+    if (a.g_log_prob) {
+      const int64_t given = a.plane[p];
+      if (given >= 0 && given < a.d) {
+        at[K] = (int)given, g[K] = a.g_log_prob[p];
+        all -= g[K];
+      }
+    }
+    const size_t hw = (size_t)a.h * a.w, o = (size_t)q.b * a.top * hw + q.r;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      at[j] = -1, g[j] = 0.f;
+      if (j >= a.top) continue;
+      at[j] = (int)a.top_plane[o + j * hw];
+      g[j] = at[j] < 0 ? 0.f : a.g_top[o + j * hw];
+      all -= g[j];
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const bool same = at[j] >= 0 && at[j] == at[K];
+      g[j] = a.scale * (same ? g[j] + g[K] : g[j]);
+      at[K] = same ? -1 : at[K];
+    }
+    g[K] *= a.scale;
+    k0 = a.scale * (ge != 0.f ? all - ge * a.entropy[p] : all);
+    k1 = -a.scale * kLn2 * ge;
+  }
+  // d: the plane, x: its score, -inf where the mask hides it
+  __device__ __forceinline__ float operator()(int d, float x) const {
+    const float l = c * (x - m) - ls2;
+    float slot = 0.f;
+#pragma unroll
+    for (int j = 0; j <= K; ++j) slot = d == at[j] ? g[j] : slot;
+    const float v = __builtin_amdgcn_exp2f(l) * (k0 + k1 * fmaxf(l, -1e4f)) + slot;
+    return x == -INFINITY ? 0.f : v;
+  }
+};
+
+// neighbouring pixels next to each other: one lane per pixel and 16 planes, blockIdx.y numbers the groups of planes
+template <typename T, int K, typename Off>
+__global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
+  constexpr int kN = 16;
+  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
+  if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const T* vol = (const T*)a.vol + offset_of(a.vs, q);
-  T* grad = (T*)a.grad + offset_of(a.gs, q);
-  const uint8_t* mask = a.mask ? a.mask + offset_of(a.ms, q) : nullptr;
-  const float m = a.row_max[p], ls = a.row_log[p], ent = a.entropy[p];
-  const bool empty = ls == -INFINITY;
-  const float ge = a.g_entropy ? a.g_entropy[p] : 0.f;
-  float all = a.g_log_sum ? a.g_log_sum[p] : 0.f;
-  int hit = -1;
-  float gl = 0.f;
-  if (a.g_log_prob) {
-    const int64_t g = a.plane[p];
-    if (g >= 0 && g < a.d) hit = (int)g, gl = a.g_log_prob[p], all -= gl;
-  }
-  int ti[DT_PLANE_MAX_TOP];
-  float tg[DT_PLANE_MAX_TOP];
-  const size_t hw = (size_t)a.h * a.w;
-  const size_t o = (size_t)q.b * a.top * hw + q.r;
+  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q), go = (Off)(offset_of(a.gs, q) * (int64_t)sizeof(T));
+  for (int d0 = blockIdx.y * kN; d0 < a.d; d0 += gridDim.y * kN) {
+    T raw[kN];
 #pragma unroll
-  for (int j = 0; j < DT_PLANE_MAX_TOP; ++j) {
-    ti[j] = -1, tg[j] = 0.f;
-    if (a.g_top && j < a.top) {
-      ti[j] = (int)a.top_plane[o + j * hw];
-      if (ti[j] >= 0) tg[j] = a.g_top[o + j * hw], all -= tg[j];
-    }
-  }
-  for (int d = 0; d < a.d; ++d) {
-    const float x = to_f32(vol[d * a.vs[1]]);
-    float g = 0.f;
-    if (!empty && !(mask && !mask[d * a.ms[1]]) && x != -INFINITY) {
-      const float lp = a.scale * (x - m) - ls;
-      const float pr = expf(lp);
-      g = pr * (all - ge * (fmaxf(lp, -1e4f) + ent));
-      if (d == hit) g += gl;
+    for (int e = 0; e < kN; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, a.d - 1) * a.vs[1], vo);
+    float x[kN];
+    if (a.mask) {
+      uint8_t seen[kN];
 #pragma unroll
-      for (int j = 0; j < DT_PLANE_MAX_TOP; ++j)
-        if (d == ti[j]) g += tg[j];
+      for (int e = 0; e < kN; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, a.d - 1) * a.ms[1], mo);
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
     }
-    grad[d * a.gs[1]] = from_f32<T>(a.scale * g);
+    const Pull<K> pull(a, p, q);
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      if (d0 + e >= a.d) break;
+      *(T*)((char*)((T*)a.grad + (d0 + e) * a.gs[1]) + go) = from_f32<T>(pull(d0 + e, x[e]));
+    }
   }
 }
 
+// the planes of a pixel next to each other, in the volume and in its gradient: G lanes per pixel, 16 bytes per lane, load and store
+template <typename T, int K, int G, typename Off>
+__global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
+  constexpr int kVec = Vec16<T>::n;
+  const int lane = threadIdx.x % G;
+  const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
+  if (p >= (uint32_t)a.b * a.h * a.w) return;
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
+  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q), go = (Off)(offset_of(a.gs, q) * (int64_t)sizeof(T));
+  const Pull<K> pull(a, p, q);
+#pragma unroll 4
+  for (int d = lane * kVec; d < a.d; d += G * kVec) {
+    if (d + kVec <= a.d) {
+      const Vec16<T> v = load<Vec16<T>>(a.vol, (Off)(vo + d * sizeof(T)));
+      Vec16<T> r;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const bool seen = !a.mask || a.mask[(d + j) * a.ms[1] + mo];
+        r.v[j] = from_f32<T>(pull(d + j, seen ? to_f32(v.v[j]) : -INFINITY));
+      }
+      *(Vec16<T>*)((char*)a.grad + (Off)(go + d * sizeof(T))) = r;
+    } else {
+      for (int e = d; e < a.d; ++e) {
+        const bool seen = !a.mask || a.mask[e * a.ms[1] + mo];
+        const float x = seen ? to_f32(load<T>(a.vol, (Off)(vo + e * sizeof(T)))) : -INFINITY;
+        *(T*)((char*)a.grad + (Off)(go + e * sizeof(T))) = from_f32<T>(pull(e, x));
+      }
+    }
+  }
+}
+
+// ---- planes of depths ------------------------------------------------------------------------------------------------------------
+// 64-bit differences of 32-bit depths are exact wherever two of them are close, so a tie is a tie; 16 planes' loads are in flight together.
 __global__ void __launch_bounds__(256) nearest_planes_kernel(PlaneNear a) {
-  const unsigned p = blockIdx.x * 256u + threadIdx.x;
-  if (p >= (unsigned)a.b * a.h * a.w) return;
+  constexpr int kN = 16;
+  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
+  if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const float* planes = a.planes + offset_of(a.ps, q);
   const float depth = a.depth[p];
   int at = -1;
-  if (depth > 0.f && depth < INFINITY) {
-    double best = INFINITY;
-    for (int d = 0; d < a.d; ++d) {
-      const double off = fabs((double)planes[d * a.ps[1]] - (double)depth);
-      if (off < best) best = off, at = d;
+  double best = INFINITY;
+  for (int d0 = 0; d0 < a.d; d0 += kN) {
+    float v[kN];
+#pragma unroll
+    for (int e = 0; e < kN; ++e) v[e] = planes[min(d0 + e, a.d - 1) * a.ps[1]];  // (the last plane again: never nearer than itself)
+#pragma unroll
+    for (int e = 0; e < kN; ++e) {
+      const double off = fabs((double)v[e] - (double)depth);
+      if (off < best) best = off, at = d0 + e;
     }
   }
-  a.out[p] = at;
+  a.out[p] = depth > 0.f && depth < INFINITY ? at : -1;
 }
 
 template <typename F>
@@ -454,17 +555,42 @@ void by_top(int top, F&& f) {
   else f(std::integral_constant<int, 8>{});
 }
 
+// bytes from the first pixel (plus `planes` planes) to the last
+int64_t span_of(const int64_t (&s)[4], int b, int h, int w, int planes, int size) {
+  return ((b - 1) * s[0] + (h - 1) * s[2] + (w - 1) * s[3] + planes * s[1]) * size;
+}
+
 template <typename T, int K>
-void launch_stats(const PlaneFwd& a, hipStream_t s) {
+void launch_stats(const PlaneFwd& a, bool wide, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
   static const int force = getenv("DT_PLANE_VAR") ? atoi(getenv("DT_PLANE_VAR")) : 0;  // EXPERIMENT
+  const dim3 block(256);
   if (a.vs[1] == 1) {
-    if (force == 16) DT_LAUNCH((plane_stats_last_kernel<T, K, 16>), dim3((pixels + 15) / 16), dim3(256), 0, s, a);
-    else if (force == 8) DT_LAUNCH((plane_stats_last_kernel<T, K, 8>), dim3((pixels + 31) / 32), dim3(256), 0, s, a);
-    else DT_LAUNCH((plane_stats_last_kernel<T, K, 4>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
+    const dim3 grid((pixels + 63) / 64);
+    if (wide) DT_LAUNCH((plane_stats_last_kernel<T, 8, 4, uint64_t>), grid, block, 0, s, a);
+    else if (force == 16) DT_LAUNCH((plane_stats_last_kernel<T, K, 16, uint32_t>), dim3((pixels + 15) / 16), block, 0, s, a);
+    else if (force == 8) DT_LAUNCH((plane_stats_last_kernel<T, K, 8, uint32_t>), dim3((pixels + 31) / 32), block, 0, s, a);
+    else DT_LAUNCH((plane_stats_last_kernel<T, K, 4, uint32_t>), grid, block, 0, s, a);
   } else {
-    if (force == 1) DT_LAUNCH((plane_stats_first_kernel<T, K, 1>), dim3((pixels + 255) / 256), dim3(256), 0, s, a);
-    else DT_LAUNCH((plane_stats_first_kernel<T, K, 4>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
+    if (wide) DT_LAUNCH((plane_stats_first_kernel<T, 8, 1, uint64_t>), dim3((pixels + 255) / 256), block, 0, s, a);
+    else if (force == 1) DT_LAUNCH((plane_stats_first_kernel<T, K, 1, uint32_t>), dim3((pixels + 255) / 256), block, 0, s, a);
+    else DT_LAUNCH((plane_stats_first_kernel<T, K, 4, uint32_t>), dim3((pixels + 63) / 64), block, 0, s, a);
+  }
+}
+
+template <typename T, int K>
+void launch_grad(const PlaneBwd& a, bool wide, hipStream_t s) {
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  static const int force = getenv("DT_PLANE_VAR") ? atoi(getenv("DT_PLANE_VAR")) : 0;  // EXPERIMENT
+  const dim3 block(256), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + 15) / 16));
+  if (a.vs[1] == 1 && a.gs[1] == 1) {
+    const dim3 grid((pixels + 63) / 64);
+    if (wide) DT_LAUNCH((plane_grad_last_kernel<T, 8, 4, uint64_t>), grid, block, 0, s, a);
+    else if (force == 16) DT_LAUNCH((plane_grad_last_kernel<T, K, 16, uint32_t>), dim3((pixels + 15) / 16), block, 0, s, a);
+    else DT_LAUNCH((plane_grad_last_kernel<T, K, 4, uint32_t>), grid, block, 0, s, a);
+  } else {
+    if (wide) DT_LAUNCH((plane_grad_first_kernel<T, 8, uint64_t>), by_pixel, block, 0, s, a);
+    else DT_LAUNCH((plane_grad_first_kernel<T, K, uint32_t>), by_pixel, block, 0, s, a);
   }
 }
 
@@ -499,7 +625,10 @@ int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint
   a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
   a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
   by_type(d->dtype, [&](auto v) {
-    by_top(d->top, [&](auto k) { launch_stats<decltype(v), k.value>(a, to_stream(s)); });
+    const int64_t limit = (int64_t)1 << 32;
+    const bool wide = span_of(a.vs, a.b, a.h, a.w, a.vs[1] == 1 ? a.d + 16 : 0, sizeof v) >= limit ||
+                      (mask && span_of(a.ms, a.b, a.h, a.w, 0, 1) >= limit);
+    by_top(d->top, [&](auto k) { launch_stats<decltype(v), k.value>(a, wide, to_stream(s)); });
   });
   return check_launch("dt_cv_plane_log_probs");
 }
@@ -516,9 +645,14 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
   for (int i = 0; i < 4; ++i) a.vs[i] = d->vol_stride[i], a.ms[i] = d->mask_stride[i], a.gs[i] = d->grad_stride[i];
   a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
   a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
-  const unsigned pixels = (unsigned)d->b * d->h * d->w;
+  if (!g_top_log_prob) a.top = 0;
   by_type(d->dtype, [&](auto v) {
-    DT_LAUNCH(plane_grad_kernel<decltype(v)>, dim3((pixels + 255) / 256), dim3(256), 0, to_stream(s), a);
+    const int64_t limit = (int64_t)1 << 32;
+    const bool last = a.vs[1] == 1 && a.gs[1] == 1;
+    const bool wide = span_of(a.vs, a.b, a.h, a.w, last ? a.d + 16 : 0, sizeof v) >= limit ||
+                      span_of(a.gs, a.b, a.h, a.w, last ? a.d + 16 : 0, sizeof v) >= limit ||
+                      (mask && span_of(a.ms, a.b, a.h, a.w, 0, 1) >= limit);
+    by_top(a.top, [&](auto k) { launch_grad<decltype(v), k.value>(a, wide, to_stream(s)); });
   });
   return check_launch("dt_cv_plane_log_probs_grad");
 }
