@@ -7,7 +7,6 @@
 #include <hip/hip_bf16.h>
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 namespace dt {
 
@@ -91,7 +90,12 @@ __device__ __forceinline__ Pixel pixel_of(uint32_t p, int h, int w, Div by_hw, D
   q.x = q.r - q.y * w;
   return q;
 }
-__device__ __forceinline__ int64_t offset_of(const int64_t (&s)[4], const Pixel& q) { return q.b * s[0] + q.y * s[2] + q.x * s[3]; }
+// elements from the tensor's first pixel to this one.  Off is 32 bits where every byte that a launch touches lies within 4 GB of its
+// tensor's first (the low words of the strides are enough then), 64 bits otherwise
+template <typename Off>
+__device__ __forceinline__ Off offset_of(const int64_t (&s)[4], const Pixel& q) {
+  return (Off)q.b * (Off)s[0] + (Off)q.y * (Off)s[2] + (Off)q.x * (Off)s[3];
+}
 
 // scale (x - m) - ls for the outputs: halves, so that two scores at opposite ends of the float range do not overflow in between
 __device__ __forceinline__ float log_prob_of(float x, float m, float ls, float scale) {
@@ -109,11 +113,16 @@ __device__ __forceinline__ double make_key(uint32_t hi, uint32_t lo) { return __
 __device__ __forceinline__ double key_of(float x, int plane) {
   const float c = x + 0.f;
   const uint32_t hi = c != c ? 0x7fe00000u : __float_as_uint(c);
-  return make_key(hi, (uint32_t)plane ^ ~(uint32_t)((int32_t)hi >> 31));
+  return make_key(hi, ~(uint32_t)plane ^ (uint32_t)((int32_t)hi >> 31));
 }
 __device__ __forceinline__ uint32_t key_hi(double k) { return (uint32_t)((uint64_t)__double_as_longlong(k) >> 32); }
 __device__ __forceinline__ int key_plane(double k) {
-  return (int)((uint32_t)__double_as_longlong(k) ^ ~(uint32_t)((int32_t)key_hi(k) >> 31));
+  return (int)~((uint32_t)__double_as_longlong(k) ^ (uint32_t)((int32_t)key_hi(k) >> 31));
+}
+// the same score, `by` planes further on
+__device__ __forceinline__ double key_moved(double k, int by) {
+  const uint32_t hi = key_hi(k), sign = (uint32_t)((int32_t)hi >> 31);
+  return make_key(hi, (uint32_t)__double_as_longlong(k) - (((uint32_t)by ^ sign) - sign));
 }
 __device__ __forceinline__ void order(double& a, double& b) {
   const double hi = fmax(a, b), lo = fmin(a, b);
@@ -148,10 +157,42 @@ __device__ __forceinline__ void merge_keys(double (&k)[K], const double (&o)[K])
       if (!(i & dist)) order(k[i], k[i + dist]);
 }
 
+// ---- exchange inside groups of G = 1, 4 neighbouring lanes ---------------------------------------------------------------------------
+template <int STEP>
+__device__ __forceinline__ uint32_t other_u32(uint32_t v) {  // lane ^ STEP
+  constexpr int ctrl = STEP == 1 ? 0xB1 : 0x4E;  // quad_perm 1,0,3,2 / 2,3,0,1
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);
+}
+template <int STEP>
+__device__ __forceinline__ float other(float v) { return __uint_as_float(other_u32<STEP>(__float_as_uint(v))); }
+template <int STEP>
+__device__ __forceinline__ double other(double v) {
+  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  return make_key(other_u32<STEP>((uint32_t)(b >> 32)), other_u32<STEP>((uint32_t)b));
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+  if constexpr (G == 4) v = fmaxf(v, other<1>(v)), v = fmaxf(v, other<2>(v));
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (G == 4) v += other<1>(v), v += other<2>(v);
+  return v;
+}
+template <int K, int STEP>
+__device__ __forceinline__ void merge_lanes(double (&k)[K]) {
+  double o[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) o[j] = other<STEP>(k[j]);
+  merge_keys(k, o);
+}
+
 // ---- running statistics of one lane --------------------------------------------------------------------------------------------
 // m: largest score so far (-inf: none); with y = c (x - m), c = scale log2 e: s = sum 2^y and t = sum 2^y y.  When the maximum moves
 // by delta = c (m_old - m_new): s' = s 2^delta, t' = (t + delta s) 2^delta.  A NaN score, or +inf (inf - inf), makes s and with it
 // every statistic NaN; the clamp keeps 0 * -inf out of t.  Differences come before the product: scores far from zero lose nothing.
+// The G lanes of a group that share a pixel move their maximum together, so that their sums need no rescaling when they join.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int K>
 struct Stats {
@@ -170,12 +211,13 @@ struct Stats {
     }
     m = to;
   }
-  // N more scores (masked ones are -inf); plane(e) numbers them in ascending order
-  template <int N, typename F>
+  // N more scores (masked ones are -inf), of planes plane(0) < plane(1) < ...
+  template <int G, int N, typename F>
   __device__ __forceinline__ void add(const float (&x)[N], float c, F plane) {
     float top = m;
 #pragma unroll
     for (int e = 0; e < N; ++e) top = fmaxf(top, x[e]);
+    top = group_max<G>(top);
     if (top != m) rebase(top, c);
     const float m0 = m == -INFINITY ? 0.f : m;
 #pragma unroll
@@ -197,48 +239,45 @@ struct Stats {
       }
     }
   }
-  __device__ __forceinline__ void join(float om, float os, float ot, const double (&ok)[K > 0 ? K : 1], float c) {
-    Stats o;
-    o.m = om, o.s = os, o.t = ot;
-    const float top = fmaxf(m, om);
-    if (top != m) rebase(top, c);
-    if (top != om) o.rebase(top, c);
-    s += o.s, t += o.t;
-    if constexpr (K > 0) merge_keys(key, ok);
-  }
 };
 
-// what a pixel's lane(s) write once its statistics are complete; lanes share the alternatives' slots (slot j belongs to lane j % lanes)
-template <int K>
-__device__ __forceinline__ void write_stats(const PlaneFwd& a, uint32_t p, const Pixel& q, const Stats<K>& st, int64_t given, float x_given,
-                                            int lane, int lanes) {
+// Writes a pixel's outputs from its statistics, which G lanes hold alike: lane 0 the real values, lane j the alternatives j, j + G, ...
+template <int K, int G, typename Off>
+__device__ __forceinline__ void write(const PlaneFwd& a, uint32_t p, const Pixel& q, const Stats<K>& st, int64_t given, float x_given, int lane) {
+  const float s = st.s, t = st.t;
   const float m = st.m == -INFINITY ? 0.f : st.m;
-  const bool empty = st.s == 0.f;
-  const float ls = logf(st.s);
+  const bool empty = s == 0.f;
+  const float ls = kLn2 * __builtin_amdgcn_logf(s);  // (s is 0, NaN or at least 1)
   if (lane == 0) {
-    a.entropy[p] = empty ? 0.f : ls - kLn2 * (st.t / st.s);
+    a.entropy[p] = empty ? 0.f : ls - kLn2 * (t * __builtin_amdgcn_rcpf(s));
     a.log_sum[p] = m * a.scale + ls;
     if (a.row_max) a.row_max[p] = m, a.row_log[p] = ls;
     if (a.plane) a.log_prob[p] = given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale);
   }
   if constexpr (K > 0) {
-    const size_t hw = (size_t)a.h * a.w;
-    const size_t o = (size_t)q.b * a.top * hw + q.r;
+    const Off hw = (Off)a.h * a.w;
+    Off o = ((Off)q.b * a.top + lane) * hw + q.r;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      if (j >= a.top) break;
-      if (lane != j % lanes) continue;
-      const bool none = key_hi(st.key[j]) == kNone;
-      const int at = key_plane(st.key[j]);
-      a.top_plane[o + j * hw] = none ? -1 : at;
-      a.top_log_prob[o + j * hw] = none ? -INFINITY : log_prob_of(__uint_as_float(key_hi(st.key[j])), m, ls, a.scale);
-      if (a.top_depth) a.top_depth[o + j * hw] = none ? 0.f : a.planes[offset_of(a.ps, q) + at * a.ps[1]];
+    for (int j = 0; j < K; j += G, o += G * hw) {
+      double k = st.key[j];
+#pragma unroll
+      for (int i = 1; i < G && j + i < K; ++i) {
+        const double other_slot = st.key[j + i];  // (read before it is chosen: a chosen read would move the list to memory)
+        k = lane == i ? other_slot : k;
+      }
+      if (j + lane >= a.top) break;
+      const bool none = key_hi(k) == kNone;
+      const int at = key_plane(k);
+      a.top_plane[o] = none ? -1 : at;
+      a.top_log_prob[o] = none ? -INFINITY : log_prob_of(__uint_as_float(key_hi(k)), m, ls, a.scale);
+      if (a.top_depth) a.top_depth[o] = none ? 0.f : a.planes[offset_of<Off>(a.ps, q) + (Off)at * (Off)a.ps[1]];
     }
   }
 }
 
-// Scores are addressed as a launch-uniform 64-bit base (scalar registers) plus an offset per lane of type Off: 32 bits where every
-// pixel lies within 4 GB of the first, which costs no vector arithmetic per load, 64 bits otherwise.
+// ---- reading scores ----------------------------------------------------------------------------------------------------------------
+// Scores are addressed as a launch-uniform 64-bit base (scalar registers) plus an offset in bytes per lane: no vector arithmetic per load
+// where Off is 32 bits.  A mask that does not vary over the planes is read once per pixel by the kernels; the readers apply one that does.
 template <typename T, typename Off>
 __device__ __forceinline__ T load(const void* base, Off off) { return *(const T*)((const char*)base + off); }
 
@@ -249,155 +288,192 @@ __device__ __forceinline__ float score_at(const PlaneFwd& a, Off vo, Off mo, int
   return seen ? to_f32(*(const T*)((const char*)a.vol + d * a.vs[1] * (int64_t)sizeof(T) + vo)) : -INFINITY;
 }
 
-// Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel, 16 planes at a time in registers,
-// all their loads in flight together (planes past the end read the last one again and count as -inf).
-// S waves of the workgroup share 64 pixels, each takes a contiguous range of planes, and the first joins the S partial results.
+// N planes d0, d0 + 1, ... of one pixel; those from `end` on count as -inf.  All loads are in flight together and none is guarded
+// (past the end the last plane is read again): a guard per load makes the compiler wait for each.
+template <typename T, int N, typename Off, typename A>
+__device__ __forceinline__ void read_first(float (&x)[N], const A& a, bool masked, int d0, int end, Off vo, Off mo) {
+  T raw[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, end - 1) * a.vs[1], vo);
+  if (masked) {
+    uint8_t seen[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, end - 1) * a.ms[1], mo);
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = to_f32(raw[e]);
+  }
+  if (d0 + N > end) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = d0 + e < end ? x[e] : -INFINITY;
+  }
+}
+
+template <typename T, int N>
+struct Vec {  // aligned like one element: global memory accesses need no more
+  T v[N];
+};
+// Layout of N planes per lane among G lanes of a pixel, from plane d0 on, 16 bytes per lane and load: plane of element e of lane 0; lane
+// l's is l * kVec further on
+template <typename T, int G>
+struct Spread {
+  static constexpr int kVec = 16 / sizeof(T), kStep = G * kVec;
+  __device__ __forceinline__ static int plane(int d0, int e) { return d0 + (e / kVec) * kStep + e % kVec; }
+};
+template <typename T, int G, int N, typename Off, typename A>
+__device__ __forceinline__ void read_last(float (&x)[N], const A& a, bool masked, int d0, int lane, Off vo, Off mo) {
+  using L = Spread<T, G>;
+  constexpr int kVec = L::kVec;
+  const Off lvo = vo + lane * 16u, lmo = mo + (Off)(lane * kVec) * (Off)a.ms[1];
+  T raw[N];
+  uint8_t seen[N];
+  if (d0 + N * G <= a.d) {
+#pragma unroll
+    for (int e = 0; e < N; e += kVec) {
+      const Vec<T, kVec> v = load<Vec<T, kVec>>((const T*)a.vol + L::plane(d0, e), lvo);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
+    }
+    if (masked && a.ms[1] == 1) {
+#pragma unroll
+      for (int e = 0; e < N; e += kVec) {
+        const Vec<uint8_t, kVec> v = load<Vec<uint8_t, kVec>>(a.mask + L::plane(d0, e), lmo);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) seen[e + j] = v.v[j];
+      }
+    } else if (masked) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) seen[e] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], lmo);
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = !masked || seen[e] ? to_f32(raw[e]) : -INFINITY;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += kVec) {
+      const int left = a.d - L::plane(d0, e) - lane * kVec;  // planes from this lane's first on
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) raw[e + j] = T();
+      if (L::plane(d0, e) + L::kStep <= a.d) {
+        const Vec<T, kVec> v = load<Vec<T, kVec>>((const T*)a.vol + L::plane(d0, e), lvo);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
+      } else if (left > 0) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) raw[e + j] = load<T>((const T*)a.vol + L::plane(d0, e), (Off)(lvo + (Off)min(j, left - 1) * (Off)sizeof(T)));
+      }
+      if (masked && left > 0) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          seen[e + j] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], (Off)(lmo + (Off)min(j, left - 1) * (Off)a.ms[1]));
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      x[e] = L::plane(d0, e) + lane * kVec < a.d && (!masked || seen[e]) ? to_f32(raw[e]) : -INFINITY;
+  }
+}
+
+// ---- statistics --------------------------------------------------------------------------------------------------------------------
+constexpr int kN = 16;  // planes per lane in registers
+
+// the first half of a lane's planes, where the second lies past the end
+template <int G, int K, typename F>
+__device__ __forceinline__ void add_planes(Stats<K>& st, const float (&x)[kN], float c, bool half, F plane) {
+  if (half) {
+    float y[kN / 2];
+#pragma unroll
+    for (int e = 0; e < kN / 2; ++e) y[e] = x[e];
+    st.template add<G>(y, c, plane);
+  } else {
+    st.template add<G>(x, c, plane);
+  }
+}
+
+// Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel.
+// S = 4: the four waves of a workgroup share 64 pixels, a quarter of the planes each; the partial results change places through LDS so
+// that four neighbouring lanes hold the four parts of a pixel, and all waves join and write 16 pixels each.
 template <typename T, int K, int S, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
-  constexpr int kPixels = 256 / S, kN = 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-  const uint32_t at = blockIdx.x * kPixels + (S == 1 ? threadIdx.x : lane);
-  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  const bool live = at < pixels;
-  const uint32_t p = live ? at : pixels - 1;
-  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q);
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w, first = blockIdx.x * (256u / S);
   const float c = a.scale * kLog2e;
-  int64_t given = -1;
-  float x_given = 0.f;
-  if (a.plane && (S == 1 || wave == 0)) {
-    given = a.plane[p];
-    if (given >= 0 && given < a.d) x_given = score_at<T>(a, vo, mo, given);
+  // the pixel this lane writes (and, S == 1, the one it reads)
+  const uint32_t at = first + threadIdx.x / S, p = min(at, pixels - 1);
+  const int group = threadIdx.x % S;
+  const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
+  const Off mo = offset_of<Off>(a.ms, q), vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T);
+  const bool masked = a.mask && a.ms[1] != 0;
+  const uint8_t seen = a.mask && !masked ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
+  const int64_t given = a.plane ? a.plane[p] : -1;
+  Off rvo = vo, rmo = mo;
+  int begin = 0, end = a.d;
+  if constexpr (S > 1) {
+    const Pixel r = pixel_of(min(first + lane, pixels - 1), a.h, a.w, a.by_hw, a.by_w);
+    rvo = offset_of<Off>(a.vs, r) * (Off)sizeof(T), rmo = offset_of<Off>(a.ms, r);
+    const int part = (a.d + S - 1) / S;
+    begin = wave * part, end = min(a.d, begin + part);
   }
-  const int part = S == 1 ? a.d : (a.d + S - 1) / S;
-  const int begin = S == 1 ? 0 : wave * part, end = min(a.d, begin + part);
   Stats<K> st;
   for (int d0 = begin; d0 < end; d0 += kN) {
-    T raw[kN];
-#pragma unroll
-    for (int e = 0; e < kN; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, end - 1) * a.vs[1], vo);
     float x[kN];
-    if (a.mask) {
-      uint8_t seen[kN];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, end - 1) * a.ms[1], mo);
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
-    }
-    if (d0 + kN > end) {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = d0 + e < end ? x[e] : -INFINITY;
-    }
-    st.add(x, c, [&](int e) { return d0 + e; });
+    read_first<T>(x, a, masked, d0, end, rvo, rmo);
+    add_planes<1>(st, x, c, d0 + kN / 2 >= end, [&](int e) { return d0 + e; });
   }
   if constexpr (S > 1) {
-    __shared__ float part_f[S - 1][3][64];
-    __shared__ double part_k[S - 1][K > 0 ? K : 1][64];
-    if (wave > 0) {
-      part_f[wave - 1][0][lane] = st.m, part_f[wave - 1][1][lane] = st.s, part_f[wave - 1][2][lane] = st.t;
+    constexpr int kRow = 64 + 16;  // (the four parts of 16 pixels fall into different banks)
+    __shared__ float part_f[3][S * kRow];
+    __shared__ double part_k[K > 0 ? K : 1][S * kRow];
+    const int put = wave * kRow + lane;
+    part_f[0][put] = st.m, part_f[1][put] = st.s, part_f[2][put] = st.t;
 #pragma unroll
-      for (int j = 0; j < K; ++j) part_k[wave - 1][j][lane] = st.key[j];
-    }
+    for (int j = 0; j < K; ++j) part_k[j][put] = st.key[j];
     __syncthreads();
-    if (wave > 0) return;
+    const int get = group * kRow + threadIdx.x / S;
+    st.m = part_f[0][get], st.s = part_f[1][get], st.t = part_f[2][get];
 #pragma unroll
-    for (int o = 0; o < S - 1; ++o) {
-      double k[K > 0 ? K : 1];
-#pragma unroll
-      for (int j = 0; j < K; ++j) k[j] = part_k[o][j][lane];
-      st.join(part_f[o][0][lane], part_f[o][1][lane], part_f[o][2][lane], k, c);
-    }
+    for (int j = 0; j < K; ++j) st.key[j] = part_k[j][get];
+    const float top = group_max<S>(st.m);
+    if (top != st.m) st.rebase(top, c);
+    st.s = group_sum<S>(st.s), st.t = group_sum<S>(st.t);
+    if constexpr (K > 0) merge_lanes<K, 1>(st.key), merge_lanes<K, 2>(st.key);
   }
-  if (live) write_stats<K>(a, p, q, st, given, x_given, 0, 1);
+  if (!seen) st = Stats<K>();
+  const float x_given = group == 0 && given >= 0 && given < a.d ? score_at<T>(a, vo, mo, given) : 0.f;
+  if (at < pixels) write<K, S, Off>(a, p, q, st, given, x_given, group);
 }
 
-// exchange with the lane of another group of 1, 2, 4 or 8 lanes of the same row of 16 (the groups' lanes hold equal values)
-template <int STEP>
-__device__ __forceinline__ uint32_t other_u32(uint32_t v) {
-  constexpr int ctrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x140;  // quad_perm 1,0,3,2 / 2,3,0,1; half mirror; mirror
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true);
-}
-template <int STEP>
-__device__ __forceinline__ float other(float v) { return __uint_as_float(other_u32<STEP>(__float_as_uint(v))); }
-template <int STEP>
-__device__ __forceinline__ double other(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
-  return make_key(other_u32<STEP>((uint32_t)(b >> 32)), other_u32<STEP>((uint32_t)b));
-}
-template <int K, int STEP>
-__device__ __forceinline__ void join_lanes(Stats<K>& st, float c) {
-  double k[K > 0 ? K : 1];
-#pragma unroll
-  for (int j = 0; j < K; ++j) k[j] = other<STEP>(st.key[j]);
-  st.join(other<STEP>(st.m), other<STEP>(st.s), other<STEP>(st.t), k, c);
-}
-
-template <typename T>
-struct Vec16 {  // 16 bytes of scores, aligned like one score: global loads need no more
-  static constexpr int n = 16 / sizeof(T);
-  T v[n];
-};
-
-// Volume with the planes of a pixel next to each other (channels_last): G lanes per pixel, 16 bytes of scores per lane and load.
-template <typename T, int K, int G, typename Off>
+// Volume with the planes of a pixel next to each other (channels_last): four lanes per pixel, 8 planes per lane at a time.
+template <typename T, int K, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
-  constexpr int kN = 16, kVec = Vec16<T>::n, kStep = G * kVec;
+  constexpr int G = 4, N = 8;
+  using L = Spread<T, G>;
   const int lane = threadIdx.x % G;
   const uint32_t at = blockIdx.x * (256u / G) + threadIdx.x / G;
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  const bool live = at < pixels;
-  const uint32_t p = live ? at : pixels - 1;
+  const uint32_t p = min(at, pixels - 1);
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q);
+  const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q);
   const float c = a.scale * kLog2e;
-  int64_t given = -1;
-  float x_given = 0.f;
-  if (a.plane) {
-    given = a.plane[p];
-    if (given >= 0 && given < a.d) x_given = score_at<T>(a, vo, mo, given);
-  }
+  const bool masked = a.mask && a.ms[1] != 0;
+  const uint8_t seen = a.mask && !masked ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
+  const int64_t given = a.plane ? a.plane[p] : -1;
   Stats<K> st;
-  for (int d0 = 0; d0 < a.d; d0 += kN * G) {
-    const bool whole = d0 + kN * G <= a.d;
-    T raw[kN];
-    auto plane = [&](int e) { return d0 + (e / kVec) * kStep + lane * kVec + e % kVec; };
-#pragma unroll
-    for (int e = 0; e < kN; e += kVec) {
-      const int d = plane(e);
-      if (whole || d + kVec <= a.d) {
-        const Vec16<T> v = load<Vec16<T>>((const T*)a.vol + d0 + (e / kVec) * kStep, (Off)(vo + lane * 16u));
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) raw[e + j] = load<T>((const T*)a.vol, (Off)(vo + min(d + j, a.d - 1) * sizeof(T)));
-      }
-    }
-    float x[kN];
-    if (a.mask) {
-      uint8_t seen[kN];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) seen[e] = a.mask[min(plane(e), a.d - 1) * a.ms[1] + mo];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
-    }
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = plane(e) < a.d ? x[e] : -INFINITY;
-    }
-    st.add(x, c, plane);
+  for (int d0 = 0; d0 < a.d; d0 += N * G) {
+    float x[N];
+    read_last<T, G>(x, a, masked, d0, lane, vo, mo);
+    st.template add<G>(x, c, [&](int e) { return L::plane(d0, e); });
   }
-  if constexpr (G >= 2) join_lanes<K, 1>(st, c);
-  if constexpr (G >= 4) join_lanes<K, 2>(st, c);
-  if constexpr (G >= 8) join_lanes<K, 4>(st, c);
-  if constexpr (G >= 16) join_lanes<K, 8>(st, c);
-  if (live) write_stats<K>(a, p, q, st, given, x_given, lane, G);
+  st.s = group_sum<G>(st.s), st.t = group_sum<G>(st.t);
+  if constexpr (K > 0) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) st.key[j] = key_moved(st.key[j], lane * L::kVec);
+    merge_lanes<K, 1>(st.key), merge_lanes<K, 2>(st.key);
+  }
+  if (!seen) st = Stats<K>();
+  const float x_given = lane == 0 && given >= 0 && given < a.d ? score_at<T>(a, vo, mo, given) : 0.f;
+  if (at < pixels) write<K, G, Off>(a, p, q, st, given, x_given, lane);
 }
 
 // ---- gradient ------------------------------------------------------------------------------------------------------------------
@@ -408,37 +484,37 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
 template <int K>
 struct Pull {
   float m, ls2, c, k0, k1;
+  bool hidden;
   int at[K + 1];
   float g[K + 1];
-  __device__ __forceinline__ Pull(const PlaneBwd& a, uint32_t p, const Pixel& q) {
-    m = a.row_max[p], ls2 = a.row_log[p] * kLog2e, c = a.scale * kLog2e;
+  __device__ __forceinline__ Pull(const PlaneBwd& a, uint32_t p, const Pixel& q, bool hidden) : hidden(hidden) {
+    // (loads first, none behind a condition on another's value)
+    m = a.row_max[p];
+    const float ls = a.row_log[p], ent = a.entropy[p];
     const float ge = a.g_entropy ? a.g_entropy[p] : 0.f;
     float all = a.g_log_sum ? a.g_log_sum[p] : 0.f;
-    at[K] = -1, g[K] = 0.f;
-    if (a.g_log_prob) {
-      const int64_t given = a.plane[p];
-      if (given >= 0 && given < a.d) {
-        at[K] = (int)given, g[K] = a.g_log_prob[p];
-        all -= g[K];
-      }
-    }
+    const int64_t given = a.g_log_prob ? a.plane[p] : -1;
+    g[K] = a.g_log_prob ? a.g_log_prob[p] : 0.f;
     const size_t hw = (size_t)a.h * a.w, o = (size_t)q.b * a.top * hw + q.r;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      at[j] = -1, g[j] = 0.f;
-      if (j >= a.top) continue;
-      at[j] = (int)a.top_plane[o + j * hw];
-      g[j] = at[j] < 0 ? 0.f : a.g_top[o + j * hw];
-      all -= g[j];
+      at[j] = j < a.top ? (int)a.top_plane[o + j * hw] : -1;
+      g[j] = j < a.top ? a.g_top[o + j * hw] : 0.f;
     }
+    const bool inside = given >= 0 && given < a.d;
+    at[K] = inside ? (int)given : -1, g[K] = inside ? g[K] : 0.f;
+    all -= g[K];
 #pragma unroll
     for (int j = 0; j < K; ++j) {
+      g[j] = at[j] < 0 ? 0.f : g[j];
+      all -= g[j];
       const bool same = at[j] >= 0 && at[j] == at[K];
       g[j] = a.scale * (same ? g[j] + g[K] : g[j]);
       at[K] = same ? -1 : at[K];
     }
     g[K] *= a.scale;
-    k0 = a.scale * (ge != 0.f ? all - ge * a.entropy[p] : all);
+    ls2 = ls * kLog2e, c = a.scale * kLog2e;
+    k0 = a.scale * (ge != 0.f ? all - ge * ent : all);
     k1 = -a.scale * kLn2 * ge;
   }
   // d: the plane, x: its score, -inf where the mask hides it
@@ -448,34 +524,27 @@ struct Pull {
 #pragma unroll
     for (int j = 0; j <= K; ++j) slot = d == at[j] ? g[j] : slot;
     const float v = __builtin_amdgcn_exp2f(l) * (k0 + k1 * fmaxf(l, -1e4f)) + slot;
-    return x == -INFINITY ? 0.f : v;
+    return hidden || x == -INFINITY ? 0.f : v;
+  }
+  // number the planes from another one
+  __device__ __forceinline__ void move(int by) {
+#pragma unroll
+    for (int j = 0; j <= K; ++j) at[j] = at[j] < 0 ? INT32_MIN : at[j] + by;
   }
 };
 
 // neighbouring pixels next to each other: one lane per pixel and 16 planes, blockIdx.y numbers the groups of planes
 template <typename T, int K, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
-  constexpr int kN = 16;
   const uint32_t p = blockIdx.x * 256u + threadIdx.x;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q), go = (Off)(offset_of(a.gs, q) * (int64_t)sizeof(T));
+  const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q), go = offset_of<Off>(a.gs, q) * (Off)sizeof(T);
+  const bool masked = a.mask && a.ms[1] != 0;
   for (int d0 = blockIdx.y * kN; d0 < a.d; d0 += gridDim.y * kN) {
-    T raw[kN];
-#pragma unroll
-    for (int e = 0; e < kN; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, a.d - 1) * a.vs[1], vo);
     float x[kN];
-    if (a.mask) {
-      uint8_t seen[kN];
-#pragma unroll
-      for (int e = 0; e < kN; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, a.d - 1) * a.ms[1], mo);
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
-    } else {
-#pragma unroll
-      for (int e = 0; e < kN; ++e) x[e] = to_f32(raw[e]);
-    }
-    const Pull<K> pull(a, p, q);
+    read_first<T>(x, a, masked, d0, a.d, vo, mo);
+    const Pull<K> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
       if (d0 + e >= a.d) break;
@@ -484,45 +553,50 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
   }
 }
 
-// the planes of a pixel next to each other, in the volume and in its gradient: G lanes per pixel, 16 bytes per lane, load and store
-template <typename T, int K, int G, typename Off>
+// the planes of a pixel next to each other, in the volume and in its gradient: four lanes per pixel, 16 bytes per lane, load and store
+template <typename T, int K, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
-  constexpr int kVec = Vec16<T>::n;
+  constexpr int G = 4;
+  using L = Spread<T, G>;
   const int lane = threadIdx.x % G;
   const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const Off vo = (Off)(offset_of(a.vs, q) * (int64_t)sizeof(T)), mo = (Off)offset_of(a.ms, q), go = (Off)(offset_of(a.gs, q) * (int64_t)sizeof(T));
-  const Pull<K> pull(a, p, q);
-#pragma unroll 4
-  for (int d = lane * kVec; d < a.d; d += G * kVec) {
-    if (d + kVec <= a.d) {
-      const Vec16<T> v = load<Vec16<T>>(a.vol, (Off)(vo + d * sizeof(T)));
-      Vec16<T> r;
+  const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q), go = offset_of<Off>(a.gs, q) * (Off)sizeof(T);
+  const bool masked = a.mask && a.ms[1] != 0;
+  float x[kN];
+  read_last<T, G>(x, a, masked, 0, lane, vo, mo);
+  Pull<K> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+  pull.move(-lane * L::kVec);
+  for (int d0 = 0;;) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const bool seen = !a.mask || a.mask[(d + j) * a.ms[1] + mo];
-        r.v[j] = from_f32<T>(pull(d + j, seen ? to_f32(v.v[j]) : -INFINITY));
-      }
-      *(Vec16<T>*)((char*)a.grad + (Off)(go + d * sizeof(T))) = r;
-    } else {
-      for (int e = d; e < a.d; ++e) {
-        const bool seen = !a.mask || a.mask[e * a.ms[1] + mo];
-        const float x = seen ? to_f32(load<T>(a.vol, (Off)(vo + e * sizeof(T)))) : -INFINITY;
-        *(T*)((char*)a.grad + (Off)(go + e * sizeof(T))) = from_f32<T>(pull(e, x));
+    for (int e = 0; e < kN; e += L::kVec) {
+      const int d = L::plane(d0, e) + lane * L::kVec;
+      Vec<T, L::kVec> r;
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) r.v[j] = from_f32<T>(pull(L::plane(d0, e + j), x[e + j]));
+      if (d + L::kVec <= a.d) {
+        *(Vec<T, L::kVec>*)((char*)((T*)a.grad + L::plane(d0, e)) + (Off)(go + lane * 16u)) = r;
+      } else {
+#pragma unroll
+        for (int j = 0; j < L::kVec; ++j)
+          if (d + j < a.d) *(T*)((char*)((T*)a.grad + L::plane(d0, e) + j) + (Off)(go + lane * 16u)) = r.v[j];
       }
     }
+    d0 += kN * G;
+    if (d0 >= a.d) break;
+    read_last<T, G>(x, a, masked, d0, lane, vo, mo);
   }
 }
 
 // ---- planes of depths ------------------------------------------------------------------------------------------------------------
 // 64-bit differences of 32-bit depths are exact wherever two of them are close, so a tie is a tie; 16 planes' loads are in flight together.
-__global__ void __launch_bounds__(256) nearest_planes_kernel(PlaneNear a) {
-  constexpr int kN = 16;
-  const uint32_t p = blockIdx.x * 256u + threadIdx.x;
+// Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 5.1 us with four).
+__global__ void __launch_bounds__(64) nearest_planes_kernel(PlaneNear a) {
+  const uint32_t p = blockIdx.x * 64u + threadIdx.x;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
-  const float* planes = a.planes + offset_of(a.ps, q);
+  const float* planes = a.planes + offset_of<int64_t>(a.ps, q);
   const float depth = a.depth[p];
   int at = -1;
   double best = INFINITY;
@@ -555,43 +629,40 @@ void by_top(int top, F&& f) {
   else f(std::integral_constant<int, 8>{});
 }
 
-// bytes from the first pixel (plus `planes` planes) to the last
-int64_t span_of(const int64_t (&s)[4], int b, int h, int w, int planes, int size) {
+// bytes from a tensor's first pixel to its last (and over `planes` planes)
+int64_t span_of(const int64_t (&s)[4], int b, int h, int w, int64_t planes, int size) {
   return ((b - 1) * s[0] + (h - 1) * s[2] + (w - 1) * s[3] + planes * s[1]) * size;
 }
+constexpr int64_t kNear = (int64_t)1 << 32;
 
 template <typename T, int K>
-void launch_stats(const PlaneFwd& a, bool wide, hipStream_t s) {
+void launch_stats(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  static const int force = getenv("DT_PLANE_VAR") ? atoi(getenv("DT_PLANE_VAR")) : 0;  // EXPERIMENT
-  const dim3 block(256);
-  if (a.vs[1] == 1) {
-    const dim3 grid((pixels + 63) / 64);
-    if (wide) DT_LAUNCH((plane_stats_last_kernel<T, 8, 4, uint64_t>), grid, block, 0, s, a);
-    else if (force == 16) DT_LAUNCH((plane_stats_last_kernel<T, K, 16, uint32_t>), dim3((pixels + 15) / 16), block, 0, s, a);
-    else if (force == 8) DT_LAUNCH((plane_stats_last_kernel<T, K, 8, uint32_t>), dim3((pixels + 31) / 32), block, 0, s, a);
-    else DT_LAUNCH((plane_stats_last_kernel<T, K, 4, uint32_t>), grid, block, 0, s, a);
-  } else {
-    if (wide) DT_LAUNCH((plane_stats_first_kernel<T, 8, 1, uint64_t>), dim3((pixels + 255) / 256), block, 0, s, a);
-    else if (force == 1) DT_LAUNCH((plane_stats_first_kernel<T, K, 1, uint32_t>), dim3((pixels + 255) / 256), block, 0, s, a);
-    else DT_LAUNCH((plane_stats_first_kernel<T, K, 4, uint32_t>), dim3((pixels + 63) / 64), block, 0, s, a);
-  }
+  const dim3 block(256), by_pixel((pixels + 255) / 256), by_four((pixels + 63) / 64);
+  // Four waves per 64 pixels pay (the exchange, four lanes writing a pixel) where few pixels with many planes would leave the chip idle.
+  // Measured us, fp32, 0 / 4 alternatives, four waves against one:
+  //   D = 16:   19200 pixels 3.5 / 4.4 against 2.8 / 3.6;  307200 pixels 13.0 / 19.1 against  6.3 /  9.4
+  //   D = 64:   76800 pixels 6.3 / 8.8 against 7.1 / 10.5; 307200 pixels 15.5 / 23.4 against 16.8 / 20.8
+  //   D = 128: 153600 pixels 15.3 / 20.0 against 15.6 / 22.2; 307200 pixels 32.8 / 40.6 against 33.0 / 37.3
+  const bool share = (int64_t)pixels < 2400 * ((int64_t)a.d - 24);
+  if (a.vs[1] == 1) DT_LAUNCH((plane_stats_last_kernel<T, K, uint32_t>), by_four, block, 0, s, a);
+  else if (share) DT_LAUNCH((plane_stats_first_kernel<T, K, 4, uint32_t>), by_four, block, 0, s, a);
+  else DT_LAUNCH((plane_stats_first_kernel<T, K, 1, uint32_t>), by_pixel, block, 0, s, a);
 }
 
-template <typename T, int K>
-void launch_grad(const PlaneBwd& a, bool wide, hipStream_t s) {
+template <typename T>
+void launch_stats_wide(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  static const int force = getenv("DT_PLANE_VAR") ? atoi(getenv("DT_PLANE_VAR")) : 0;  // EXPERIMENT
-  const dim3 block(256), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + 15) / 16));
-  if (a.vs[1] == 1 && a.gs[1] == 1) {
-    const dim3 grid((pixels + 63) / 64);
-    if (wide) DT_LAUNCH((plane_grad_last_kernel<T, 8, 4, uint64_t>), grid, block, 0, s, a);
-    else if (force == 16) DT_LAUNCH((plane_grad_last_kernel<T, K, 16, uint32_t>), dim3((pixels + 15) / 16), block, 0, s, a);
-    else DT_LAUNCH((plane_grad_last_kernel<T, K, 4, uint32_t>), grid, block, 0, s, a);
-  } else {
-    if (wide) DT_LAUNCH((plane_grad_first_kernel<T, 8, uint64_t>), by_pixel, block, 0, s, a);
-    else DT_LAUNCH((plane_grad_first_kernel<T, K, uint32_t>), by_pixel, block, 0, s, a);
-  }
+  if (a.vs[1] == 1) DT_LAUNCH((plane_stats_last_kernel<T, 8, int64_t>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
+  else DT_LAUNCH((plane_stats_first_kernel<T, 8, 1, int64_t>), dim3((pixels + 255) / 256), dim3(256), 0, s, a);
+}
+
+template <typename T, int K, typename Off>
+void launch_grad(const PlaneBwd& a, hipStream_t s) {
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  const dim3 block(256), by_four((pixels + 63) / 64), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + kN - 1) / kN));
+  if (a.vs[1] == 1 && a.gs[1] == 1) DT_LAUNCH((plane_grad_last_kernel<T, K, Off>), by_four, block, 0, s, a);
+  else DT_LAUNCH((plane_grad_first_kernel<T, K, Off>), by_pixel, block, 0, s, a);
 }
 
 int check_desc(const char* what, const dt_plane_desc* d) {
@@ -625,10 +696,12 @@ int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint
   a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
   a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
   by_type(d->dtype, [&](auto v) {
-    const int64_t limit = (int64_t)1 << 32;
-    const bool wide = span_of(a.vs, a.b, a.h, a.w, a.vs[1] == 1 ? a.d + 16 : 0, sizeof v) >= limit ||
-                      (mask && span_of(a.ms, a.b, a.h, a.w, 0, 1) >= limit);
-    by_top(d->top, [&](auto k) { launch_stats<decltype(v), k.value>(a, wide, to_stream(s)); });
+    const bool last = a.vs[1] == 1;
+    if (span_of(a.vs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear || (mask && span_of(a.ms, a.b, a.h, a.w, last ? a.d : 0, 1) >= kNear) ||
+        (a.top_depth && span_of(a.ps, a.b, a.h, a.w, a.d, 4) >= kNear) || (int64_t)a.b * a.top * a.h * a.w >= kNear / 8)
+      launch_stats_wide<decltype(v)>(a, to_stream(s));
+    else
+      by_top(a.top, [&](auto k) { launch_stats<decltype(v), k.value>(a, to_stream(s)); });
   });
   return check_launch("dt_cv_plane_log_probs");
 }
@@ -647,12 +720,12 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
   a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
   if (!g_top_log_prob) a.top = 0;
   by_type(d->dtype, [&](auto v) {
-    const int64_t limit = (int64_t)1 << 32;
     const bool last = a.vs[1] == 1 && a.gs[1] == 1;
-    const bool wide = span_of(a.vs, a.b, a.h, a.w, last ? a.d + 16 : 0, sizeof v) >= limit ||
-                      span_of(a.gs, a.b, a.h, a.w, last ? a.d + 16 : 0, sizeof v) >= limit ||
-                      (mask && span_of(a.ms, a.b, a.h, a.w, 0, 1) >= limit);
-    by_top(a.top, [&](auto k) { launch_grad<decltype(v), k.value>(a, wide, to_stream(s)); });
+    const bool wide = span_of(a.vs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear ||
+                      span_of(a.gs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear ||
+                      (mask && span_of(a.ms, a.b, a.h, a.w, last ? a.d : 0, 1) >= kNear);
+    if (wide) launch_grad<decltype(v), 8, int64_t>(a, to_stream(s));
+    else by_top(a.top, [&](auto k) { launch_grad<decltype(v), k.value, uint32_t>(a, to_stream(s)); });
   });
   return check_launch("dt_cv_plane_log_probs_grad");
 }
@@ -667,7 +740,7 @@ int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, 
   a.b = b, a.d = d, a.h = h, a.w = w;
   a.by_hw = make_div((uint32_t)h * w), a.by_w = make_div(w);
   const unsigned pixels = (unsigned)b * h * w;
-  DT_LAUNCH(nearest_planes_kernel, dim3((pixels + 255) / 256), dim3(256), 0, to_stream(s), a);
+  DT_LAUNCH(nearest_planes_kernel, dim3((pixels + 63) / 64), dim3(64), 0, to_stream(s), a);
   return check_launch("dt_cv_nearest_planes_f32");
 }
 
