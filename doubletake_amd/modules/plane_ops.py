@@ -41,14 +41,16 @@ def _require_gpu(t, name):
 
 def _broadcast(t, shape, device, name):
     """``t`` as a view of ``shape`` = (b, D, h, w) with stride 0 along the axes it is broadcast over."""
-    if t.dim() != 4 or any(n != m and n != 1 for n, m in zip(t.shape, shape)):
-        raise ValueError(f"{name} {tuple(t.shape)} does not broadcast to {tuple(shape)}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.shape == shape:
+        return t
+    if t.dim() != 4 or any(n != m and n != 1 for n, m in zip(t.shape, shape)):
+        raise ValueError(f"{name} {tuple(t.shape)} does not broadcast to {tuple(shape)}")
     return t.expand(shape)
 
 
-def _desc(vol, top, scale, mask, planes, grad=None):
+def _desc(vol, top, scale, mask, planes):
     d = _abi.PlaneDesc()
     d.b, d.d, d.h, d.w = vol.shape
     d.dtype, d.top, d.scale = _DTYPES[vol.dtype], top, scale
@@ -57,51 +59,78 @@ def _desc(vol, top, scale, mask, planes, grad=None):
         d.mask_stride[:] = mask.stride()
     if planes is not None:
         d.planes_stride[:] = planes.stride()
-    if grad is not None:
-        d.grad_stride[:] = grad.stride()
     return d
 
 
 def _forward(vol, plane, top, scale, mask, planes, for_grad):
+    """(outputs, row statistics [2, b, h, w] or None, descriptor, stream)"""
     b, _, h, w = vol.shape
-    f32 = lambda *shape: torch.empty(shape, device=vol.device, dtype=torch.float32)
-    ent, lsum = f32(b, h, w), f32(b, h, w)
-    lp = f32(b, h, w) if plane is not None else None
-    tlp = f32(b, top, h, w) if top else None
-    tpl = torch.empty((b, top, h, w), device=vol.device, dtype=torch.int64) if top else None
-    tdep = f32(b, top, h, w) if planes is not None else None
-    rmax, rlog = (f32(b, h, w), f32(b, h, w)) if for_grad else (None, None)
+    ent = torch.empty((b, h, w), device=vol.device, dtype=torch.float32)
+    lsum = torch.empty_like(ent)
+    lp = torch.empty_like(ent) if plane is not None else None
+    tlp = tpl = tdep = rows = None
+    if top:
+        tlp = torch.empty((b, top, h, w), device=vol.device, dtype=torch.float32)
+        tpl = torch.empty_like(tlp, dtype=torch.int64)
+        if planes is not None:
+            tdep = torch.empty_like(tlp)
+    rmax = rlog = None
+    if for_grad:
+        rows = torch.empty((2, b, h, w), device=vol.device, dtype=torch.float32)
+        rmax = rows.data_ptr()
+        rlog = rmax + 4 * b * h * w
+    desc = _desc(vol, top, scale, mask, planes)
+    stream = _abi.current_stream(vol.device)
     if b * h * w:
         p = _abi.ptr
         _abi.check(_abi.lib().dt_cv_plane_log_probs(
-            C.byref(_desc(vol, top, scale, mask, planes)), p(vol), p(mask), p(plane), p(planes), p(lp), p(ent), p(lsum), p(tlp), p(tpl),
-            p(tdep), p(rmax), p(rlog), _abi.current_stream(vol.device)), "dt_cv_plane_log_probs")
-    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rmax, rlog
+            desc, vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
+            stream), "dt_cv_plane_log_probs")
+    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, desc, stream
+
+
+def _dense_f32(g):
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
+def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
+    vol, plane, mask, ent, tpl = ctx.saved_tensors
+    g_lp, g_ent, g_lsum, g_top = _dense_f32(g_lp), _dense_f32(g_ent), _dense_f32(g_lsum), _dense_f32(g_top)
+    grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
+    n = ent.numel()
+    if n:
+        p, desc = _abi.ptr, ctx.desc
+        desc.grad_stride[:] = grad.stride()
+        rmax = ctx.rows.data_ptr()
+        _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
+            desc, vol.data_ptr(), p(mask), p(plane), ent.data_ptr(), p(tpl), rmax, rmax + 4 * n, p(g_lp), p(g_ent), p(g_lsum), p(g_top),
+            grad.data_ptr(), ctx.stream), "dt_cv_plane_log_probs_grad")
+    return grad, None, None, None, None, None
 
 
 class _PlaneLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, vol, plane, top, scale, mask, planes):
-        out, rmax, rlog = _forward(vol, plane, top, scale, mask, planes, True)
+        out, rows, desc, stream = _forward(vol, plane, top, scale, mask, planes, True)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*[t for t in (out.top_plane_bkhw, out.top_depth_bkhw) if t is not None])
-        ctx.save_for_backward(vol, plane, mask, out.entropy_bhw, out.top_plane_bkhw, rmax, rlog)
-        ctx.top, ctx.scale = top, scale
+        if top:
+            ctx.mark_non_differentiable(*[t for t in out[4:] if t is not None])
+        ctx.save_for_backward(vol, plane, mask, out[1], out[4])
+        # made here, neither inputs nor outputs.  The engine runs a backward on the stream its forward ran on: the handle is kept, asking
+        # for it in the engine's thread costs 6 us
+        ctx.rows, ctx.desc, ctx.stream = rows, desc, stream
         return tuple(out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
-        vol, plane, mask, ent, tpl, rmax, rlog = ctx.saved_tensors
-        dense = lambda g: None if g is None else g.to(torch.float32).contiguous()
-        g_lp, g_ent, g_lsum, g_top = dense(g_lp), dense(g_ent), dense(g_lsum), dense(g_top)
-        grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
-        if vol.numel():
-            p = _abi.ptr
-            _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
-                C.byref(_desc(vol, ctx.top, ctx.scale, mask, None, grad)), p(vol), p(mask), p(plane), p(ent), p(tpl), p(rmax), p(rlog),
-                p(g_lp), p(g_ent), p(g_lsum), p(g_top), p(grad), _abi.current_stream(vol.device)), "dt_cv_plane_log_probs_grad")
-        return grad, None, None, None, None, None
+    def backward(ctx, *grads):
+        if torch.is_grad_enabled():  # create_graph=True: a second derivative raises where it is asked for (the wrapper costs 9 us)
+            return _backward_once(ctx, *grads)
+        return _backward(ctx, *grads)
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=None, depth_planes_bdhw=None) -> PlaneLogProbs:
@@ -145,7 +174,10 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
             raise ValueError(f"plane_bhw {tuple(plane.shape)} does not match the volume's pixels {(b, h, w)}")
         if plane.device != vol.device:
             raise ValueError(f"plane_bhw is on {plane.device}, expected {vol.device}")
-        plane = plane.to(torch.int64).contiguous()
+        if plane.dtype != torch.int64:
+            plane = plane.to(torch.int64)
+        if not plane.is_contiguous():
+            plane = plane.contiguous()
     mask = mask_bdhw
     if mask is not None:
         if mask.dtype != torch.bool:
@@ -184,7 +216,7 @@ def nearest_planes(depth_bhw, depth_planes_bdhw):
         raise ValueError(f"depth_bhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
     planes = _broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw")
     _require_gpu(depth, "depth_bhw")
-    depth = depth.to(torch.float32).contiguous()
+    depth = _dense_f32(depth)
     out = torch.empty((b, h, w), device=depth.device, dtype=torch.int64)
     if out.numel():
         _abi.check(_abi.lib().dt_cv_nearest_planes_f32(_abi.ptr(depth), _abi.ptr(planes), (C.c_int64 * 4)(*planes.stride()), b, D, h, w,
