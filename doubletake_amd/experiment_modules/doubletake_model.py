@@ -16,6 +16,7 @@ import torch
 import torch.nn as nn
 
 from ..modules import conv_ops as ops
+from ..modules import plane_ops
 from ..modules.cost_volume import CostVolumeManager, FeatureMeshHintVolumeManager, FeatureVolumeManager
 from ..modules.networks import CVEncoder, DepthDecoderPP, ResnetMatchingEncoder
 from ..modules.networks_fast import SkipDecoderRegression
@@ -321,9 +322,43 @@ class _HotPathDepthModel(nn.Module):
         if second is not None:
             second(tag)
 
+    def enable_plane_statistics(self, on=True, top=4, scale=1.0):
+        """Add what the cost volume says about its own answer to the outputs of ``forward`` / ``forward_from_features``
+        (CostVolumeManager.plane_statistics; no reference counterpart), all float32 at the volume's resolution:
+
+          plane_log_prob_bhw         log probability of the depth plane the predicted depth falls on
+          plane_entropy_bhw          entropy of the distribution over planes, nats: 0 = one plane, log D = no plane stands out
+          plane_top_log_prob_bkhw,   the ``top`` most probable planes and their depths (top > 0)
+          plane_top_depth_bkhw
+
+        ``scale``: factor on the volume's scores in front of the softmax.  Two more launches per call; works under captured graphs and
+        launch programs.  ``loops`` can mask depths by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
+        top, scale = int(top), float(scale)
+        if on and not 0 <= top <= min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins):
+            raise ValueError(f"top={top} not in 0..{min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins)}")
+        if on and not 0.0 < scale < float("inf"):
+            raise ValueError(f"scale={scale} must be positive and finite")
+        self._plane_statistics = (top, scale) if on else None
+        return self
+
+    def _add_plane_statistics(self, outputs, cost_volume, planes):
+        top, scale = self._plane_statistics
+        b, _, h, w = cost_volume.shape
+        for key in (f"depth_pred_s{i}_b1hw" for i in range(4)):  # the output scale that has the volume's resolution
+            depth = outputs.get(key)
+            if depth is not None and depth.shape == (b, 1, h, w):
+                break
+        else:
+            raise ValueError(f"no predicted depth at the cost volume's resolution {h}x{w}: plane statistics need one")
+        r = self.cost_volume.plane_statistics(cost_volume, planes, depth[:, 0], top=top, scale=scale)
+        outputs["plane_log_prob_bhw"], outputs["plane_entropy_bhw"] = r.log_prob_bhw, r.entropy_bhw
+        if top:
+            outputs["plane_top_log_prob_bkhw"], outputs["plane_top_depth_bkhw"] = r.top_log_prob_bkhw, r.top_depth_bkhw
+        return outputs
+
     def _launch_config(self):
         cv = self.cost_volume
-        return ops.launch_config() + (getattr(cv, "precision", None), getattr(cv, "use_span_plan", None),
+        return ops.launch_config() + (getattr(self, "_plane_statistics", None), getattr(cv, "precision", None), getattr(cv, "use_span_plan", None),
                                       getattr(cv, "channels_last_output", None))
 
     def enable_launch_programs(self, on=True):
@@ -448,7 +483,7 @@ class _HotPathDepthModel(nn.Module):
                   return_mask=return_mask)
         if isinstance(self.cost_volume, FeatureMeshHintVolumeManager):  # the other managers take no hints
             kw["cv_depth_hint_dict"] = cv_depth_hint_dict
-        cost_volume, lowest_cost, overall_mask = self.volume_stage(kw)
+        cost_volume, lowest_cost, planes, overall_mask = self.cost_volume(**kw)
         # graph mode: the replay is split here so that the hook below runs between the halves -- only when a hook is
         # waiting at capture time (every cut is one more hipGraphLaunch per replay)
         if "after_volume" in self.__dict__ or _graphs.recording():
@@ -459,7 +494,10 @@ class _HotPathDepthModel(nn.Module):
             # and all of its LDS) and beside the conv stack that follows (latency-bound, most of the chip idle):
             # loops.matching_lookahead encodes the next frame's keyframe here
             hook()
-        return self.network_stage(cur_feats, cost_volume, lowest_cost, overall_mask)
+        outputs = self.network_stage(cur_feats, cost_volume, lowest_cost, overall_mask)
+        if getattr(self, "_plane_statistics", None) is not None:
+            self._add_plane_statistics(outputs, cost_volume, planes)
+        return outputs
 
     # The two halves of the forward pass, callable on their own so that a driver with several keyframes in flight can order
     # them across HIP streams (bench.py --schedule phased): the volume kernel owns every CU and all of its LDS, the conv

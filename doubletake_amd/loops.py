@@ -83,9 +83,10 @@ class FrameTimer:
         return formats.write_scores_json(filepath, exp_name, metrics_name, scores)
 
 
-def _depth_for_fusion(outputs, size, mask_pred_depth=False, per_view_mask=True):
+def _depth_for_fusion(outputs, size, mask_pred_depth=False, per_view_mask=True, min_plane_log_prob=None):
     """Nearest upsampling of depth_pred_s0 to the ground-truth depth size and the optional masking
-    (test_incremental.py:290-294,331-352; test_offline_two_pass.py:97-117)."""
+    (test_incremental.py:290-294,331-352; test_offline_two_pass.py:97-117).  min_plane_log_prob: depths whose plane the cost
+    volume gives a lower log probability (or NaN) are masked too (``model.enable_plane_statistics``)."""
     depth = outputs["depth_pred_s0_b1hw"]
     if size is not None and tuple(depth.shape[-2:]) != tuple(size):
         depth = F.interpolate(depth, size=tuple(size), mode="nearest")
@@ -97,6 +98,12 @@ def _depth_for_fusion(outputs, size, mask_pred_depth=False, per_view_mask=True):
             m = F.interpolate(m.view(m.shape[0], 1, *m.shape[-2:]), size=depth.shape[-2:], mode="nearest").bool()
         depth = depth.clone()
         depth[~m] = -1
+    if min_plane_log_prob is not None:
+        lp = outputs.get("plane_log_prob_bhw")
+        if lp is None:
+            raise ValueError("min_plane_log_prob needs plane_log_prob_bhw among the model's outputs: model.enable_plane_statistics()")
+        lp = F.interpolate(lp.unsqueeze(1), size=depth.shape[-2:], mode="nearest")
+        depth = torch.where(lp >= min_plane_log_prob, depth, torch.full_like(depth, -1))
     return depth
 
 
@@ -124,11 +131,12 @@ class IncrementalScan:
     streams (different scans do not depend on each other; the frames of one scan do).  Arguments: see run_incremental_scan."""
 
     def __init__(self, model_fn, fuser, batches, render_hw, fuse_size=None, fused_hint=True, mask_pred_depth=False,
-                 on_frame=None, timer: FrameTimer | None = None, lookahead=None):
+                 on_frame=None, timer: FrameTimer | None = None, lookahead=None, min_plane_log_prob=None):
         self.model_fn, self.fuser = model_fn, fuser
         self.H2, self.W2 = render_hw
         self.fuse_size, self.fused_hint, self.mask_pred_depth = fuse_size, fused_hint, mask_pred_depth
         self.on_frame, self.timer, self.lookahead = on_frame, timer, lookahead
+        self.min_plane_log_prob = min_plane_log_prob
         self.renderer = None if fused_hint else MeshDepthRenderer(self.H2, self.W2)
         self.frames = 0
         self._it = iter(batches)
@@ -173,7 +181,8 @@ class IncrementalScan:
     @torch.no_grad()
     def finish_frame(self, cur_data, outputs):
         """Fuse the frame's prediction into the scan's TSDF (nearest upsampling / masking as the drivers do) and count it."""
-        depth = _depth_for_fusion(outputs, self.fuse_size, self.mask_pred_depth, per_view_mask=True)
+        depth = _depth_for_fusion(outputs, self.fuse_size, self.mask_pred_depth, per_view_mask=True,
+                                  min_plane_log_prob=self.min_plane_log_prob)
         self.fuser.fuse_frames(depth, cur_data["K_full_depth_b44"], cur_data["cam_T_world_b44"], None)
         i = self.frames
         self.frames += 1
@@ -215,7 +224,7 @@ class IncrementalScan:
 
 
 def run_incremental_scan(model_fn, fuser, batches, render_hw, fuse_size=None, fused_hint=True, mask_pred_depth=False,
-                         on_frame=None, timer: FrameTimer | None = None, lookahead=None):
+                         on_frame=None, timer: FrameTimer | None = None, lookahead=None, min_plane_log_prob=None):
     """One scan of the incremental (online) mode; batch size 1 (reference test_incremental.py:25).
 
     batches: iterable of (cur_data, src_data); cur_data carries K_s0_b44 / invK_s0_b44 / cam_T_world_b44 /
@@ -225,9 +234,12 @@ def run_incremental_scan(model_fn, fuser, batches, render_hw, fuse_size=None, fu
     reference-shaped sequence over a merged mesh.  timer: a FrameTimer that receives hint_time / model_time per frame
     (test_incremental.py:205,256-258,274-288).  lookahead: callable(next_cur_data, next_src_data) run before the model of
     the current frame -- work of frame t+1 that does not depend on frame t's result (``matching_lookahead``: its matching
-    features) and can fill the chip beside frame t's latency-bound kernels.  Returns the number of frames fused."""
+    features) and can fill the chip beside frame t's latency-bound kernels.  min_plane_log_prob: depths whose plane the cost
+    volume gives a lower log probability are not fused (needs ``model.enable_plane_statistics()``).  Returns the number of
+    frames fused."""
     scan = IncrementalScan(model_fn, fuser, batches, render_hw, fuse_size=fuse_size, fused_hint=fused_hint,
-                           mask_pred_depth=mask_pred_depth, on_frame=on_frame, timer=timer, lookahead=lookahead)
+                           mask_pred_depth=mask_pred_depth, on_frame=on_frame, timer=timer, lookahead=lookahead,
+                           min_plane_log_prob=min_plane_log_prob)
     while scan.step():
         pass
     return scan.frames
@@ -416,7 +428,7 @@ def hints_from_mesh(mesh, hint_fuser, renderer, cur_data, render_hw, hint_world_
 
 
 def two_pass_fns(model_fn, load_batch, render_hw, fuse_size=None, mask_pred_depth=False, on_frame=None,
-                 load_first_pass_batch=None, hint_world_T_world_144=None, timer: FrameTimer | None = None):
+                 load_first_pass_batch=None, hint_world_T_world_144=None, timer: FrameTimer | None = None, min_plane_log_prob=None):
     """(first_pass_fn, between_passes, second_pass_fn) for ``parallel.run_two_pass`` (``in_flight=4`` there runs the keyframe
     batches of both passes through ``parallel.KeyframePipeline``; with ``model.enable_launch_programs()`` the outputs of
     ``model_fn`` are lane-static buffers, which the step functions below consume before they return).
@@ -424,7 +436,8 @@ def two_pass_fns(model_fn, load_batch, render_hw, fuse_size=None, mask_pred_dept
     ``load_batch(i) -> (cur_data, src_data)`` fetches keyframe batch i onto this rank's GPU (only called for the
     rank's own batches).  Second-pass hints: ``hints_from_mesh``.  ``load_first_pass_batch`` / ``hint_world_T_world_144``
     serve ``revisit_fns`` (first pass over another scan; hints through a rigid transform).  timer: second-pass
-    hint_time / model_time per frame (test_offline_two_pass.py:313,360-362,371-377)."""
+    hint_time / model_time per frame (test_offline_two_pass.py:313,360-362,371-377).  min_plane_log_prob: as
+    run_incremental_scan, in both passes."""
     H2, W2 = render_hw
     load_first = load_first_pass_batch if load_first_pass_batch is not None else load_batch
 
@@ -444,7 +457,7 @@ def two_pass_fns(model_fn, load_batch, render_hw, fuse_size=None, mask_pred_dept
             empty[(b, dev)] = maps
         cur_data.update(maps)
         out = model_fn(cur_data, src_data)
-        return _depth_for_fusion(out, fuse_size, mask_pred_depth, per_view_mask=False), cur_data["K_full_depth_b44"], \
+        return _depth_for_fusion(out, fuse_size, mask_pred_depth, False, min_plane_log_prob), cur_data["K_full_depth_b44"], \
             cur_data["cam_T_world_b44"]
 
     def between(hint_fuser):
@@ -466,14 +479,14 @@ def two_pass_fns(model_fn, load_batch, render_hw, fuse_size=None, mask_pred_dept
             timer.stop("model_time", b)
         if on_frame is not None:
             on_frame(i, cur_data, out)
-        return _depth_for_fusion(out, fuse_size, mask_pred_depth, per_view_mask=False), cur_data["K_full_depth_b44"], \
+        return _depth_for_fusion(out, fuse_size, mask_pred_depth, False, min_plane_log_prob), cur_data["K_full_depth_b44"], \
             cur_data["cam_T_world_b44"]
 
     return first, between, second
 
 
 def revisit_fns(model_fn, load_first_scan_batch, load_batch, first_scan_T_second_scan_144, render_hw, fuse_size=None,
-                mask_pred_depth=False, on_frame=None, timer: FrameTimer | None = None):
+                mask_pred_depth=False, on_frame=None, timer: FrameTimer | None = None, min_plane_log_prob=None):
     """The revisit flow of reference test_revisit.py:104-260 as the step functions of ``parallel.run_two_pass``
     (``num_first_batches=`` gives the first scan's batch count):
 
@@ -488,4 +501,4 @@ def revisit_fns(model_fn, load_first_scan_batch, load_batch, first_scan_T_second
     ``first_scan_T_second_scan_144``: [1,4,4], the inverse of the rescan transform the 3RScan metadata lists (:112-114)."""
     return two_pass_fns(model_fn, load_batch, render_hw, fuse_size=fuse_size, mask_pred_depth=mask_pred_depth,
                         on_frame=on_frame, load_first_pass_batch=load_first_scan_batch,
-                        hint_world_T_world_144=first_scan_T_second_scan_144, timer=timer)
+                        hint_world_T_world_144=first_scan_T_second_scan_144, timer=timer, min_plane_log_prob=min_plane_log_prob)

@@ -162,3 +162,21 @@ def test_reference_gradient_matches_autograd_and_differences():
         d = torch.zeros_like(x)
         d.view(-1)[k] = eps
         assert abs(float((loss(x + d) - loss(x - d)) / (2 * eps) - want.view(-1)[k])) < 1e-7
+
+
+def test_model_refuses_bad_statistics_settings_and_loops_need_them():
+    from doubletake_amd import loops
+    from doubletake_amd.experiment_modules.doubletake_model import DepthModelCVHint
+
+    m = DepthModelCVHint(64, 96, matching_num_depth_bins=6, model_num_views=3, matching_encoder_type=None)
+    for kw in (dict(top=7), dict(top=-1), dict(scale=0.0), dict(scale=math.inf), dict(scale=math.nan)):
+        with pytest.raises(ValueError):
+            m.enable_plane_statistics(**kw)
+    assert m.enable_plane_statistics(top=6) is m and m._launch_config() != m.enable_plane_statistics(False)._launch_config()
+    depth = torch.ones(1, 1, 4, 6)
+    with pytest.raises(ValueError, match="enable_plane_statistics"):
+        loops._depth_for_fusion({"depth_pred_s0_b1hw": depth}, None, min_plane_log_prob=-1.0)
+    lp = torch.tensor([[[-0.5, -2.0, math.nan], [-1.0, 0.0, -math.inf]]])
+    got = loops._depth_for_fusion({"depth_pred_s0_b1hw": depth, "plane_log_prob_bhw": lp}, None, min_plane_log_prob=-1.0)
+    want = torch.tensor([[1.0, -1, -1], [1, 1, -1]]).repeat_interleave(2, 0).repeat_interleave(2, 1)
+    assert torch.equal(got[0, 0], want) and bool((depth == 1).all())
