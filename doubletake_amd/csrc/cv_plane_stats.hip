@@ -667,12 +667,16 @@ void launch_grad(const PlaneBwd& a, hipStream_t s) {
 
 int check_desc(const char* what, const dt_plane_desc* d) {
   DT_REQUIRE(d, "%s: null descriptor", what);
-  DT_REQUIRE(d->b > 0 && d->d > 0 && d->h > 0 && d->w > 0, "%s: bad extents b=%d d=%d h=%d w=%d", what, d->b, d->d, d->h, d->w);
+  DT_REQUIRE(d->b > 0 && d->d > 0 && d->d <= DT_PLANE_MAX_PLANES && d->h > 0 && d->w > 0, "%s: bad extents b=%d d=%d h=%d w=%d", what, d->b, d->d, d->h, d->w);
   DT_REQUIRE((int64_t)d->b * d->h < INT32_MAX && (int64_t)d->b * d->h * d->w < INT32_MAX, "%s: more than 2^31 - 1 pixels", what);
   DT_REQUIRE(d->dtype == DT_VOL_F32 || d->dtype == DT_VOL_F16 || d->dtype == DT_VOL_BF16, "%s: unknown dtype %d", what, d->dtype);
   DT_REQUIRE(d->top >= 0 && d->top <= DT_PLANE_MAX_TOP && d->top <= d->d, "%s: top=%d not in 0..%d", what, d->top,
              d->d < DT_PLANE_MAX_TOP ? d->d : DT_PLANE_MAX_TOP);
-  DT_REQUIRE(d->scale > 0.f && std::isfinite(d->scale), "%s: scale=%g is not positive and finite", what, (double)d->scale);
+  // (scale log2 e and the gradient's scale * g * log probability have to be finite)
+  DT_REQUIRE(d->scale >= 0.999e-30f && d->scale <= 1.001e30f, "%s: scale=%g not in 1e-30..1e30", what, (double)d->scale);
+  for (int i = 0; i < 4; ++i)
+    DT_REQUIRE(d->vol_stride[i] >= 0 && d->mask_stride[i] >= 0 && d->planes_stride[i] >= 0 && d->grad_stride[i] >= 0,
+               "%s: negative stride", what);
   return 0;
 }
 
@@ -732,11 +736,14 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
 
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
                              int w, int64_t* plane_bhw, dt_stream_t s) {
-  DT_REQUIRE(b > 0 && d > 0 && h > 0 && w > 0, "dt_cv_nearest_planes_f32: bad extents b=%d d=%d h=%d w=%d", b, d, h, w);
+  DT_REQUIRE(b > 0 && d > 0 && d <= DT_PLANE_MAX_PLANES && h > 0 && w > 0, "dt_cv_nearest_planes_f32: bad extents b=%d d=%d h=%d w=%d", b, d, h, w);
   DT_REQUIRE((int64_t)b * h < INT32_MAX && (int64_t)b * h * w < INT32_MAX, "dt_cv_nearest_planes_f32: more than 2^31 - 1 pixels");
   DT_REQUIRE(depth_bhw && depth_planes && planes_stride4 && plane_bhw, "dt_cv_nearest_planes_f32: null pointer");
   PlaneNear a{depth_bhw, depth_planes, plane_bhw};
-  for (int i = 0; i < 4; ++i) a.ps[i] = planes_stride4[i];
+  for (int i = 0; i < 4; ++i) {
+    DT_REQUIRE(planes_stride4[i] >= 0, "dt_cv_nearest_planes_f32: negative stride");
+    a.ps[i] = planes_stride4[i];
+  }
   a.b = b, a.d = d, a.h = h, a.w = w;
   a.by_hw = make_div((uint32_t)h * w), a.by_w = make_div(w);
   const unsigned pixels = (unsigned)b * h * w;

@@ -336,8 +336,8 @@ class _HotPathDepthModel(nn.Module):
         top, scale = int(top), float(scale)
         if on and not 0 <= top <= min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins):
             raise ValueError(f"top={top} not in 0..{min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins)}")
-        if on and not 0.0 < scale < float("inf"):
-            raise ValueError(f"scale={scale} must be positive and finite")
+        if on:
+            plane_ops.check_scale(scale)
         self._plane_statistics = (top, scale) if on else None
         return self
 

@@ -22,6 +22,10 @@ from .. import _abi
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 #: most alternatives per pixel (DT_PLANE_MAX_TOP)
 MAX_TOP = 8
+#: factors on the scores; the gradient's intermediate values (scale * gradient * log probability) stay finite for gradients up to 1e4
+MIN_SCALE, MAX_SCALE = 1e-30, 1e30
+#: planes per volume (DT_PLANE_MAX_PLANES)
+MAX_PLANES = 1 << 30
 
 
 class PlaneLogProbs(NamedTuple):
@@ -32,6 +36,11 @@ class PlaneLogProbs(NamedTuple):
     top_log_prob_bkhw: Optional[torch.Tensor]   # descending
     top_plane_bkhw: Optional[torch.Tensor]      # int64, as indices_to_disparity takes them; -1 where there is none
     top_depth_bkhw: Optional[torch.Tensor]
+
+
+def check_scale(scale):
+    if not MIN_SCALE <= scale <= MAX_SCALE:
+        raise ValueError(f"scale={scale} must be a positive number between {MIN_SCALE} and {MAX_SCALE}")
 
 
 def _require_gpu(t, name):
@@ -50,7 +59,7 @@ def _broadcast(t, shape, device, name):
     return t.expand(shape)
 
 
-def _desc(vol, top, scale, mask, planes):
+def _desc(vol, top, scale, mask, planes, grad=None):
     d = _abi.PlaneDesc()
     d.b, d.d, d.h, d.w = vol.shape
     d.dtype, d.top, d.scale = _DTYPES[vol.dtype], top, scale
@@ -59,11 +68,13 @@ def _desc(vol, top, scale, mask, planes):
         d.mask_stride[:] = mask.stride()
     if planes is not None:
         d.planes_stride[:] = planes.stride()
+    if grad is not None:
+        d.grad_stride[:] = grad.stride()
     return d
 
 
 def _forward(vol, plane, top, scale, mask, planes, for_grad):
-    """(outputs, row statistics [2, b, h, w] or None, descriptor, stream)"""
+    """(outputs, row statistics [2, b, h, w] or None, stream)"""
     b, _, h, w = vol.shape
     ent = torch.empty((b, h, w), device=vol.device, dtype=torch.float32)
     lsum = torch.empty_like(ent)
@@ -79,14 +90,13 @@ def _forward(vol, plane, top, scale, mask, planes, for_grad):
         rows = torch.empty((2, b, h, w), device=vol.device, dtype=torch.float32)
         rmax = rows.data_ptr()
         rlog = rmax + 4 * b * h * w
-    desc = _desc(vol, top, scale, mask, planes)
     stream = _abi.current_stream(vol.device)
     if b * h * w:
         p = _abi.ptr
         _abi.check(_abi.lib().dt_cv_plane_log_probs(
-            desc, vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
+            _desc(vol, top, scale, mask, planes), vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
             stream), "dt_cv_plane_log_probs")
-    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, desc, stream
+    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, stream
 
 
 def _dense_f32(g):
@@ -101,8 +111,9 @@ def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
     grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
     n = ent.numel()
     if n:
-        p, desc = _abi.ptr, ctx.desc
-        desc.grad_stride[:] = grad.stride()
+        # (strides are taken here: hooks on saved tensors may bring a tensor back in another layout than it was saved in)
+        p, desc = _abi.ptr, _desc(vol, ctx.top, ctx.scale, mask, None, grad)
+        plane, ent, tpl = [t if t is None or t.is_contiguous() else t.contiguous() for t in (plane, ent, tpl)]
         rmax = ctx.rows.data_ptr()
         _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
             desc, vol.data_ptr(), p(mask), p(plane), ent.data_ptr(), p(tpl), rmax, rmax + 4 * n, p(g_lp), p(g_ent), p(g_lsum), p(g_top),
@@ -113,14 +124,14 @@ def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
 class _PlaneLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, vol, plane, top, scale, mask, planes):
-        out, rows, desc, stream = _forward(vol, plane, top, scale, mask, planes, True)
+        out, rows, stream = _forward(vol, plane, top, scale, mask, planes, True)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(*[t for t in out[4:] if t is not None])
         ctx.save_for_backward(vol, plane, mask, out[1], out[4])
         # made here, neither inputs nor outputs.  The engine runs a backward on the stream its forward ran on: the handle is kept, asking
         # for it in the engine's thread costs 6 us
-        ctx.rows, ctx.desc, ctx.stream = rows, desc, stream
+        ctx.rows, ctx.stream, ctx.top, ctx.scale = rows, stream, top, scale
         return tuple(out)
 
     @staticmethod
@@ -140,7 +151,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
     plane_bhw: plane indices [b, h, w] (int64 or int32) whose log probability is wanted; one outside 0..D-1 (-1: no depth there)
         scores 0 and takes no part in the gradient.
     top: how many of the most probable planes to return, 0..min(D, 8); equal scores in the order of their planes.
-    scale: factor on the scores in front of the softmax (inverse temperature), a positive number.
+    scale: factor on the scores in front of the softmax (inverse temperature), a positive number, 1e-30..1e30.
     mask_bdhw: bool, broadcastable to the volume; False leaves a plane out, whatever the volume holds there.  A pixel without a
         visible plane of a score above -inf has entropy 0, log_sum and log_prob -inf, no alternatives (plane -1, log probability -inf,
         depth 0) and gradient 0.
@@ -156,16 +167,15 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
     if vol.dtype not in _DTYPES:
         raise ValueError(f"volume_bdhw is {vol.dtype}; float32, float16 and bfloat16 are supported")
     b, D, h, w = vol.shape
-    if D < 1:
-        raise ValueError("volume_bdhw has no planes")
+    if not 1 <= D <= MAX_PLANES:
+        raise ValueError(f"volume_bdhw has {D} planes; 1..{MAX_PLANES} are supported")
     if b * h * w >= 2**31 - 1:
         raise ValueError(f"volume_bdhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
     top = int(top)
     if not 0 <= top <= min(D, MAX_TOP):
         raise ValueError(f"top={top} not in 0..{min(D, MAX_TOP)}")
     scale = float(scale)
-    if not (0.0 < scale <= 3.4e38):
-        raise ValueError(f"scale={scale} must be positive and finite")
+    check_scale(scale)
     plane = plane_bhw
     if plane is not None:
         if plane.dtype not in (torch.int64, torch.int32):
@@ -206,8 +216,8 @@ def nearest_planes(depth_bhw, depth_planes_bdhw):
         raise ValueError(f"depth_bhw must be [b, h, w], got {tuple(depth.shape)}")
     if not depth.is_floating_point():
         raise ValueError(f"depth_bhw is {depth.dtype}; metric depths are floating point")
-    if planes.dim() != 4 or planes.shape[1] < 1:
-        raise ValueError(f"depth_planes_bdhw must be [b, D, h, w], got {tuple(planes.shape)}")
+    if planes.dim() != 4 or not 1 <= planes.shape[1] <= MAX_PLANES:
+        raise ValueError(f"depth_planes_bdhw must be [b, D, h, w] with 1..{MAX_PLANES} planes, got {tuple(planes.shape)}")
     if planes.dtype != torch.float32:
         raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
     b, h, w = depth.shape

@@ -217,14 +217,15 @@ int dt_cv_overall_mask_u8(const float* params, const float* depth_planes_bdhw, u
  *   - equal scores: the lowest plane first; alternatives beyond the planes with probability: plane -1, log prob -inf, depth 0. */
 enum { DT_VOL_F32 = 0, DT_VOL_F16 = 1, DT_VOL_BF16 = 2 };
 #define DT_PLANE_MAX_TOP 8
+#define DT_PLANE_MAX_PLANES (1 << 30)
 
 typedef struct dt_plane_desc {
-  int b, d, h, w;             /* extents of the volume; b * h * w < 2^31 */
+  int b, d, h, w;             /* extents of the volume; b * h * w < 2^31 - 1, d <= DT_PLANE_MAX_PLANES */
   int dtype;                  /* DT_VOL_*: type of the volume and of its gradient */
   int top;                    /* alternatives per pixel, 0..min(d, DT_PLANE_MAX_TOP) */
-  float scale;                /* inverse temperature, > 0 and finite */
+  float scale;                /* inverse temperature, 1e-30..1e30 */
   int pad;
-  int64_t vol_stride[4];      /* elements between neighbours along b, d, y, x: any layout */
+  int64_t vol_stride[4];      /* elements between neighbours along b, d, y, x: any layout, none negative */
   int64_t mask_stride[4];     /* bytes, likewise; 0 along a broadcast axis */
   int64_t planes_stride[4];   /* elements of the depth planes, likewise */
   int64_t grad_stride[4];     /* elements of the gradient written by ..._grad; the other call ignores it */

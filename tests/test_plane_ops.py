@@ -32,6 +32,9 @@ def _refusals():
         "scale negative": (v, dict(scale=-1.0)),
         "scale nan": (v, dict(scale=math.nan)),
         "scale inf": (v, dict(scale=math.inf)),
+        "scale too large": (v, dict(scale=2e30)),
+        "scale too small": (v, dict(scale=1e-31)),
+        "too many planes": (torch.zeros(1).expand(1, (1 << 30) + 1, 1, 1), {}),
         "plane float": (v, dict(plane_bhw=i.float())),
         "plane shape": (v, dict(plane_bhw=i[:, None])),
         "plane size": (v, dict(plane_bhw=i[:1])),
@@ -105,6 +108,9 @@ def _call_grad(d, **kw):
 
 @pytest.mark.parametrize("bad", [dict(b=0), dict(d=0), dict(h=-1), dict(w=0), dict(dtype=3), dict(dtype=-1), dict(top=5), dict(top=9, d=20),
                                  dict(top=-1), dict(scale=0.0), dict(scale=-2.0), dict(scale=math.inf), dict(scale=math.nan),
+                                 dict(scale=2e30), dict(scale=1e-31), dict(d=(1 << 30) + 1),
+                                 dict(vol_stride=(C.c_int64 * 4)(1, -1, 1, 1)), dict(mask_stride=(C.c_int64 * 4)(1, 1, -1, 1)),
+                                 dict(planes_stride=(C.c_int64 * 4)(-1, 1, 1, 1)), dict(grad_stride=(C.c_int64 * 4)(1, 1, 1, -1)),
                                  dict(b=1 << 15, h=1 << 15, w=2)])
 def test_abi_refuses_descriptors(bad):
     assert _call(_desc(**bad)) != 0 and _abi.lib().dt_last_error()
@@ -122,7 +128,7 @@ def test_abi_refuses_pointers():
         assert _call_grad(_desc(), **kw) != 0, kw
     L, st = _abi.lib(), (C.c_int64 * 4)(4, 1, 0, 0)
     for args in ((None, 16, st, 1, 4, 2, 2, 16), (16, None, st, 1, 4, 2, 2, 16), (16, 16, None, 1, 4, 2, 2, 16), (16, 16, st, 1, 4, 2, 2, None),
-                 (16, 16, st, 0, 4, 2, 2, 16), (16, 16, st, 1, 0, 2, 2, 16), (16, 16, st, 1 << 15, 4, 1 << 15, 2, 16)):
+                 (16, 16, (C.c_int64 * 4)(4, 1, -1, 0), 1, 4, 2, 2, 16), (16, 16, st, 1, (1 << 30) + 1, 2, 2, 16), (16, 16, st, 0, 4, 2, 2, 16), (16, 16, st, 1, 0, 2, 2, 16), (16, 16, st, 1 << 15, 4, 1 << 15, 2, 16)):
         assert L.dt_cv_nearest_planes_f32(*args, None) != 0, args
 
 

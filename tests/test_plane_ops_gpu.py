@@ -204,6 +204,38 @@ def test_gradient_of_several_calls_accumulates():
     assert torch.equal(leaf.grad, one + one)
 
 
+@pytest.mark.parametrize("view", ["crop last", "plane step last", "broadcast planes", "whole last"])
+def test_gradient_with_saved_tensors_kept_on_the_host(view):
+    """Hooks on saved tensors may bring the volume and the mask back dense where they were views: other strides, same values."""
+    vol, m, plane, _ = make((2, 20, 9, 11), mask="plane", seed=45)
+    v = {"crop last": vol[:, :, 1:-2, 3:-1], "plane step last": vol[:, 1::3], "broadcast planes": vol[:, :1].expand(2, 7, 9, 11),
+         "whole last": vol}[view]
+    b, D, h, w = v.shape
+    plane = plane[:, :h, :w].contiguous().clamp(max=D - 1)
+    mask = m[:, :D, :h, :w]
+    leaf = v.detach().requires_grad_(True)
+    grads = []
+    for host in (False, True):
+        if host:
+            with torch.autograd.graph.save_on_cpu():
+                r = plane_ops.plane_log_probs(leaf, plane, top=2, mask_bdhw=mask)
+        else:
+            r = plane_ops.plane_log_probs(leaf, plane, top=2, mask_bdhw=mask)
+        g, = torch.autograd.grad(r.entropy_bhw.sum() + r.top_log_prob_bkhw[:, 0].nan_to_num(neginf=0.0).sum(), leaf)
+        grads.append(g)
+    assert torch.equal(grads[0], grads[1])
+
+
+def test_scales_at_the_ends_of_their_range():
+    vol, m, plane, _ = make((1, 12, 5, 7), mask="plane", seed=46)
+    for scale in (1e-30, 1e30):   # (beyond them the call is refused)
+        r = plane_ops.plane_log_probs(vol, plane, top=3, scale=scale, mask_bdhw=m)
+        ref.check_stats(r, vol, plane, 3, scale, m)
+        leaf = (vol / scale if scale > 1 else vol).detach().requires_grad_(True)   # (sizes whose gradient is a number)
+        r = plane_ops.plane_log_probs(leaf, plane, scale=scale, mask_bdhw=m)
+        assert bool(torch.isfinite(torch.autograd.grad(r.entropy_bhw.sum(), leaf)[0]).all())
+
+
 def test_no_gradient_where_none_is_asked_for():
     vol, _, plane, planes = make((1, 9, 4, 5))
     leaf = vol.requires_grad_(True)
