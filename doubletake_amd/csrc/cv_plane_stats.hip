@@ -97,6 +97,24 @@ __device__ __forceinline__ Off offset_of(const int64_t (&s)[4], const Pixel& q) 
   return (Off)q.b * (Off)s[0] + (Off)q.y * (Off)s[2] + (Off)q.x * (Off)s[3];
 }
 
+// A launch-uniform 64-bit base plus an offset in bytes per lane.  The empty statement keeps the base in scalar registers: left to itself
+// the compiler adds the two first, a 64-bit vector addition and two registers per access, and hoists the sums out of the loop over
+// planes.  Planes innermost, D = 64, 4 alternatives, 8 x 120 x 160 pixels: 80 -> 54 registers, 13.6 -> 12.9 us.  (Not where a lane steps
+// over planes, the hoisted addresses win there: 128 planes of float16, 8 x 240 x 320 pixels 36.4 us, kept in scalar registers 39.9.)
+#define DT_GLOBAL __attribute__((address_space(1)))
+template <typename T, typename Off>
+__device__ __forceinline__ T load(const void* base, Off off) {
+  uint64_t address = (uint64_t)base;
+  if constexpr (sizeof(Off) == 4) asm("" : "+s"(address));
+  return *(const T*)(const DT_GLOBAL char*)(address + off);
+}
+template <typename T, typename Off>
+__device__ __forceinline__ void store(void* base, Off off, T v) {
+  uint64_t address = (uint64_t)base;
+  if constexpr (sizeof(Off) == 4) asm("" : "+s"(address));
+  *(T*)(DT_GLOBAL char*)(address + off) = v;
+}
+
 // scale (x - m) - ls for the outputs: halves, so that two scores at opposite ends of the float range do not overflow in between
 __device__ __forceinline__ float log_prob_of(float x, float m, float ls, float scale) {
   return 2.f * ((0.5f * x - 0.5f * m) * scale) - ls;
@@ -248,11 +266,12 @@ __device__ __forceinline__ void write(const PlaneFwd& a, uint32_t p, const Pixel
   const float m = st.m == -INFINITY ? 0.f : st.m;
   const bool empty = s == 0.f;
   const float ls = kLn2 * __builtin_amdgcn_logf(s);  // (s is 0, NaN or at least 1)
+  const Off po = (Off)p * 4;
   if (lane == 0) {
-    a.entropy[p] = empty ? 0.f : ls - kLn2 * (t * __builtin_amdgcn_rcpf(s));
-    a.log_sum[p] = m * a.scale + ls;
-    if (a.row_max) a.row_max[p] = m, a.row_log[p] = ls;
-    if (a.plane) a.log_prob[p] = given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale);
+    store(a.entropy, po, empty ? 0.f : ls - kLn2 * (t * __builtin_amdgcn_rcpf(s)));
+    store(a.log_sum, po, m * a.scale + ls);
+    if (a.row_max) store(a.row_max, po, m), store(a.row_log, po, ls);
+    if (a.plane) store(a.log_prob, po, given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale));
   }
   if constexpr (K > 0) {
     const Off hw = (Off)a.h * a.w;
@@ -268,24 +287,30 @@ __device__ __forceinline__ void write(const PlaneFwd& a, uint32_t p, const Pixel
       if (j + lane >= a.top) break;
       const bool none = key_hi(k) == kNone;
       const int at = key_plane(k);
-      a.top_plane[o] = none ? -1 : at;
-      a.top_log_prob[o] = none ? -INFINITY : log_prob_of(__uint_as_float(key_hi(k)), m, ls, a.scale);
-      if (a.top_depth) a.top_depth[o] = none ? 0.f : a.planes[offset_of<Off>(a.ps, q) + (Off)at * (Off)a.ps[1]];
+      store<int64_t>(a.top_plane, o * 8, none ? -1 : at);
+      store(a.top_log_prob, o * 4, none ? -INFINITY : log_prob_of(__uint_as_float(key_hi(k)), m, ls, a.scale));
+      if (a.top_depth) {
+        const float depth = none ? 0.f : load<float>(a.planes, (Off)((offset_of<Off>(a.ps, q) + (Off)at * (Off)a.ps[1]) * 4));
+        store(a.top_depth, o * 4, depth);
+      }
     }
   }
 }
 
 // ---- reading scores ----------------------------------------------------------------------------------------------------------------
-// Scores are addressed as a launch-uniform 64-bit base (scalar registers) plus an offset in bytes per lane: no vector arithmetic per load
-// where Off is 32 bits.  A mask that does not vary over the planes is read once per pixel by the kernels; the readers apply one that does.
-template <typename T, typename Off>
-__device__ __forceinline__ T load(const void* base, Off off) { return *(const T*)((const char*)base + off); }
+// A mask that does not vary over the planes is read once per pixel by the kernels; the readers apply one that does.
 
 // the score of one plane of a pixel, -inf where the mask hides it
 template <typename T, typename Off>
-__device__ __forceinline__ float score_at(const PlaneFwd& a, Off vo, Off mo, int64_t d) {
+__device__ __forceinline__ float score_first(const PlaneFwd& a, Off vo, Off mo, int64_t d) {
   const bool seen = !a.mask || a.mask[d * a.ms[1] + mo];
   return seen ? to_f32(*(const T*)((const char*)a.vol + d * a.vs[1] * (int64_t)sizeof(T) + vo)) : -INFINITY;
+}
+
+template <typename T, typename Off>
+__device__ __forceinline__ float score_last(const PlaneFwd& a, Off vo, Off mo, int d) {
+  const bool seen = !a.mask || load<uint8_t>(a.mask, (Off)(mo + (Off)d * (Off)a.ms[1]));
+  return seen ? to_f32(load<T>(a.vol, (Off)(vo + (Off)d * (Off)sizeof(T)))) : -INFINITY;
 }
 
 // N planes d0, d0 + 1, ... of one pixel; those from `end` on count as -inf.  All loads are in flight together and none is guarded
@@ -293,12 +318,14 @@ __device__ __forceinline__ float score_at(const PlaneFwd& a, Off vo, Off mo, int
 template <typename T, int N, typename Off, typename A>
 __device__ __forceinline__ void read_first(float (&x)[N], const A& a, bool masked, int d0, int end, Off vo, Off mo) {
   T raw[N];
+  const char* vol = (const char*)a.vol + vo;
+  const uint8_t* mask = a.mask + mo;
 #pragma unroll
-  for (int e = 0; e < N; ++e) raw[e] = load<T>((const T*)a.vol + min(d0 + e, end - 1) * a.vs[1], vo);
+  for (int e = 0; e < N; ++e) raw[e] = ((const T*)vol)[min(d0 + e, end - 1) * a.vs[1]];
   if (masked) {
     uint8_t seen[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) seen[e] = load<uint8_t>(a.mask + min(d0 + e, end - 1) * a.ms[1], mo);
+    for (int e = 0; e < N; ++e) seen[e] = mask[min(d0 + e, end - 1) * a.ms[1]];
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
   } else {
@@ -406,7 +433,7 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   const Off mo = offset_of<Off>(a.ms, q), vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T);
   const bool masked = a.mask && a.ms[1] != 0;
   const uint8_t seen = a.mask && !masked ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
-  const int64_t given = a.plane ? a.plane[p] : -1;
+  const int64_t given = a.plane ? load<int64_t>(a.plane, (Off)p * 8) : -1;
   Off rvo = vo, rmo = mo;
   int begin = 0, end = a.d;
   if constexpr (S > 1) {
@@ -440,7 +467,7 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
     if constexpr (K > 0) merge_lanes<K, 1>(st.key), merge_lanes<K, 2>(st.key);
   }
   if (!seen) st = Stats<K>();
-  const float x_given = group == 0 && given >= 0 && given < a.d ? score_at<T>(a, vo, mo, given) : 0.f;
+  const float x_given = group == 0 && given >= 0 && given < a.d ? score_first<T>(a, vo, mo, given) : 0.f;
   if (at < pixels) write<K, S, Off>(a, p, q, st, given, x_given, group);
 }
 
@@ -458,7 +485,7 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   const float c = a.scale * kLog2e;
   const bool masked = a.mask && a.ms[1] != 0;
   const uint8_t seen = a.mask && !masked ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
-  const int64_t given = a.plane ? a.plane[p] : -1;
+  const int64_t given = a.plane ? load<int64_t>(a.plane, (Off)p * 8) : -1;
   Stats<K> st;
   for (int d0 = 0; d0 < a.d; d0 += N * G) {
     float x[N];
@@ -472,7 +499,7 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
     merge_lanes<K, 1>(st.key), merge_lanes<K, 2>(st.key);
   }
   if (!seen) st = Stats<K>();
-  const float x_given = lane == 0 && given >= 0 && given < a.d ? score_at<T>(a, vo, mo, given) : 0.f;
+  const float x_given = lane == 0 && given >= 0 && given < a.d ? score_last<T>(a, vo, mo, (int)given) : 0.f;
   if (at < pixels) write<K, G, Off>(a, p, q, st, given, x_given, lane);
 }
 
@@ -481,7 +508,7 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
 //   dx = 2^l (k0 + k1 max(l, -1e4)) + (gradient of the slot that names the plane),
 //   k0 = scale (g_log_sum - g_log_prob - sum g_top - g_entropy entropy), k1 = -scale g_entropy ln 2.
 // Slots: the alternatives and the given plane, which is folded into the alternative it coincides with; all planes differ.
-template <int K>
+template <int K, typename Off>
 struct Pull {
   float m, ls2, c, k0, k1;
   bool hidden;
@@ -489,17 +516,18 @@ struct Pull {
   float g[K + 1];
   __device__ __forceinline__ Pull(const PlaneBwd& a, uint32_t p, const Pixel& q, bool hidden) : hidden(hidden) {
     // (loads first, none behind a condition on another's value)
-    m = a.row_max[p];
-    const float ls = a.row_log[p], ent = a.entropy[p];
-    const float ge = a.g_entropy ? a.g_entropy[p] : 0.f;
-    float all = a.g_log_sum ? a.g_log_sum[p] : 0.f;
-    const int64_t given = a.g_log_prob ? a.plane[p] : -1;
-    g[K] = a.g_log_prob ? a.g_log_prob[p] : 0.f;
-    const size_t hw = (size_t)a.h * a.w, o = (size_t)q.b * a.top * hw + q.r;
+    const Off po = (Off)p * 4;
+    m = load<float>(a.row_max, po);
+    const float ls = load<float>(a.row_log, po), ent = load<float>(a.entropy, po);
+    const float ge = a.g_entropy ? load<float>(a.g_entropy, po) : 0.f;
+    float all = a.g_log_sum ? load<float>(a.g_log_sum, po) : 0.f;
+    const int64_t given = a.g_log_prob ? load<int64_t>(a.plane, po * 2) : -1;
+    g[K] = a.g_log_prob ? load<float>(a.g_log_prob, po) : 0.f;
+    const Off hw = (Off)a.h * a.w, o = (Off)q.b * a.top * hw + q.r;
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      at[j] = j < a.top ? (int)a.top_plane[o + j * hw] : -1;
-      g[j] = j < a.top ? a.g_top[o + j * hw] : 0.f;
+      at[j] = j < a.top ? (int)load<int64_t>(a.top_plane, (Off)((o + j * hw) * 8)) : -1;
+      g[j] = j < a.top ? load<float>(a.g_top, (Off)((o + j * hw) * 4)) : 0.f;
     }
     const bool inside = given >= 0 && given < a.d;
     at[K] = inside ? (int)given : -1, g[K] = inside ? g[K] : 0.f;
@@ -544,11 +572,12 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
   for (int d0 = blockIdx.y * kN; d0 < a.d; d0 += gridDim.y * kN) {
     float x[kN];
     read_first<T>(x, a, masked, d0, a.d, vo, mo);
-    const Pull<K> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+    const Pull<K, Off> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+    T* grad = (T*)((char*)a.grad + go);
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
       if (d0 + e >= a.d) break;
-      *(T*)((char*)((T*)a.grad + (d0 + e) * a.gs[1]) + go) = from_f32<T>(pull(d0 + e, x[e]));
+      grad[(d0 + e) * a.gs[1]] = from_f32<T>(pull(d0 + e, x[e]));
     }
   }
 }
@@ -566,7 +595,7 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
   const bool masked = a.mask && a.ms[1] != 0;
   float x[kN];
   read_last<T, G>(x, a, masked, 0, lane, vo, mo);
-  Pull<K> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+  Pull<K, Off> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
   pull.move(-lane * L::kVec);
   for (int d0 = 0;;) {
 #pragma unroll
@@ -576,11 +605,11 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
 #pragma unroll
       for (int j = 0; j < L::kVec; ++j) r.v[j] = from_f32<T>(pull(L::plane(d0, e + j), x[e + j]));
       if (d + L::kVec <= a.d) {
-        *(Vec<T, L::kVec>*)((char*)((T*)a.grad + L::plane(d0, e)) + (Off)(go + lane * 16u)) = r;
+        store((T*)a.grad + L::plane(d0, e), (Off)(go + lane * 16u), r);
       } else {
 #pragma unroll
         for (int j = 0; j < L::kVec; ++j)
-          if (d + j < a.d) *(T*)((char*)((T*)a.grad + L::plane(d0, e) + j) + (Off)(go + lane * 16u)) = r.v[j];
+          if (d + j < a.d) store((T*)a.grad + L::plane(d0, e) + j, (Off)(go + lane * 16u), r.v[j]);
       }
     }
     d0 += kN * G;
@@ -702,7 +731,7 @@ int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint
   by_type(d->dtype, [&](auto v) {
     const bool last = a.vs[1] == 1;
     if (span_of(a.vs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear || (mask && span_of(a.ms, a.b, a.h, a.w, last ? a.d : 0, 1) >= kNear) ||
-        (a.top_depth && span_of(a.ps, a.b, a.h, a.w, a.d, 4) >= kNear) || (int64_t)a.b * a.top * a.h * a.w >= kNear / 8)
+        (a.top_depth && span_of(a.ps, a.b, a.h, a.w, a.d, 4) >= kNear) || (int64_t)a.b * std::max(a.top, 1) * a.h * a.w >= kNear / 8)
       launch_stats_wide<decltype(v)>(a, to_stream(s));
     else
       by_top(a.top, [&](auto k) { launch_stats<decltype(v), k.value>(a, to_stream(s)); });
@@ -727,7 +756,8 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
     const bool last = a.vs[1] == 1 && a.gs[1] == 1;
     const bool wide = span_of(a.vs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear ||
                       span_of(a.gs, a.b, a.h, a.w, last ? a.d : 0, sizeof v) >= kNear ||
-                      (mask && span_of(a.ms, a.b, a.h, a.w, last ? a.d : 0, 1) >= kNear);
+                      (mask && span_of(a.ms, a.b, a.h, a.w, last ? a.d : 0, 1) >= kNear) ||
+                      (int64_t)a.b * std::max(a.top, 1) * a.h * a.w >= kNear / 8;
     if (wide) launch_grad<decltype(v), 8, int64_t>(a, to_stream(s));
     else by_top(a.top, [&](auto k) { launch_grad<decltype(v), k.value, uint32_t>(a, to_stream(s)); });
   });
