@@ -313,24 +313,42 @@ __device__ __forceinline__ float score_last(const PlaneFwd& a, Off vo, Off mo, i
   return seen ? to_f32(load<T>(a.vol, (Off)(vo + (Off)d * (Off)sizeof(T)))) : -INFINITY;
 }
 
+struct __attribute__((packed)) Packed4 {
+  uint32_t bytes;
+};
+template <typename T, int N>
+struct Vec {  // aligned like one element: global memory accesses need no more
+  T v[N];
+};
+// N planes' scores and mask bytes as they come from memory.  Loading and unpacking are apart so that other work goes in between.
+template <typename T, int N>
+struct Raw {
+  T v[N];
+  uint8_t seen[N];
+  uint32_t word[N / 4];
+};
+
 // N planes d0, d0 + 1, ... of one pixel; those from `end` on count as -inf.  All loads are in flight together and none is guarded
 // (past the end the last plane is read again): a guard per load makes the compiler wait for each.
 template <typename T, int N, typename Off, typename A>
-__device__ __forceinline__ void read_first(float (&x)[N], const A& a, bool masked, int d0, int end, Off vo, Off mo) {
-  T raw[N];
+__device__ __forceinline__ void load_first(Raw<T, N>& raw, const A& a, bool masked, int d0, int end, Off vo, Off mo) {
   const char* vol = (const char*)a.vol + vo;
   const uint8_t* mask = a.mask + mo;
 #pragma unroll
-  for (int e = 0; e < N; ++e) raw[e] = ((const T*)vol)[min(d0 + e, end - 1) * a.vs[1]];
+  for (int e = 0; e < N; ++e) raw.v[e] = ((const T*)vol)[min(d0 + e, end - 1) * a.vs[1]];
   if (masked) {
-    uint8_t seen[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) seen[e] = mask[min(d0 + e, end - 1) * a.ms[1]];
+    for (int e = 0; e < N; ++e) raw.seen[e] = mask[min(d0 + e, end - 1) * a.ms[1]];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack_first(float (&x)[N], const Raw<T, N>& raw, bool masked, int d0, int end) {
+  if (masked) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = seen[e] ? to_f32(raw[e]) : -INFINITY;
+    for (int e = 0; e < N; ++e) x[e] = raw.seen[e] ? to_f32(raw.v[e]) : -INFINITY;
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = to_f32(raw[e]);
+    for (int e = 0; e < N; ++e) x[e] = to_f32(raw.v[e]);
   }
   if (d0 + N > end) {
 #pragma unroll
@@ -338,10 +356,6 @@ __device__ __forceinline__ void read_first(float (&x)[N], const A& a, bool maske
   }
 }
 
-template <typename T, int N>
-struct Vec {  // aligned like one element: global memory accesses need no more
-  T v[N];
-};
 // Layout of N planes per lane among G lanes of a pixel, from plane d0 on, 16 bytes per lane and load: plane of element e of lane 0; lane
 // l's is l * kVec further on
 template <typename T, int G>
@@ -349,56 +363,69 @@ struct Spread {
   static constexpr int kVec = 16 / sizeof(T), kStep = G * kVec;
   __device__ __forceinline__ static int plane(int d0, int e) { return d0 + (e / kVec) * kStep + e % kVec; }
 };
-template <typename T, int G, int N, typename Off, typename A>
-__device__ __forceinline__ void read_last(float (&x)[N], const A& a, bool masked, int d0, int lane, Off vo, Off mo) {
+// What the readers below know about the mask at compile time: none that varies over the planes, one byte per load, or the planes' bytes
+// next to each other like the scores (a comparison of a channels_last volume): then as many bytes per load as scores, taken apart when
+// they are used.  One kernel for all three held the addresses and branches of each: 4 alternatives, 8 x 64 x 120 x 160: 14.8 us, 13.6 apart.
+enum MaskKind { kNoMask, kMaskBytes, kMaskVectors };
+template <MaskKind M, typename T, int G, int N, typename Off, typename A>
+__device__ __forceinline__ void load_last(Raw<T, N>& raw, const A& a, int d0, int lane, Off vo, Off mo) {
   using L = Spread<T, G>;
   constexpr int kVec = L::kVec;
   const Off lvo = vo + lane * 16u, lmo = mo + (Off)(lane * kVec) * (Off)a.ms[1];
-  T raw[N];
-  uint8_t seen[N];
   if (d0 + N * G <= a.d) {
 #pragma unroll
     for (int e = 0; e < N; e += kVec) {
       const Vec<T, kVec> v = load<Vec<T, kVec>>((const T*)a.vol + L::plane(d0, e), lvo);
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
+      for (int j = 0; j < kVec; ++j) raw.v[e + j] = v.v[j];
     }
-    if (masked && a.ms[1] == 1) {
+    if constexpr (M == kMaskVectors) {
 #pragma unroll
       for (int e = 0; e < N; e += kVec) {
-        const Vec<uint8_t, kVec> v = load<Vec<uint8_t, kVec>>(a.mask + L::plane(d0, e), lmo);
+        const Vec<Packed4, kVec / 4> v = load<Vec<Packed4, kVec / 4>>(a.mask + L::plane(d0, e), lmo);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) seen[e + j] = v.v[j];
+        for (int j = 0; j < kVec / 4; ++j) raw.word[e / 4 + j] = v.v[j].bytes;
       }
-    } else if (masked) {
+    } else if constexpr (M == kMaskBytes) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) seen[e] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], lmo);
+      for (int e = 0; e < N; ++e) raw.seen[e] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], lmo);
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = !masked || seen[e] ? to_f32(raw[e]) : -INFINITY;
   } else {
 #pragma unroll
     for (int e = 0; e < N; e += kVec) {
       const int left = a.d - L::plane(d0, e) - lane * kVec;  // planes from this lane's first on
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) raw[e + j] = T();
+      for (int j = 0; j < kVec; ++j) raw.v[e + j] = T(), raw.seen[e + j] = 0;
       if (L::plane(d0, e) + L::kStep <= a.d) {
         const Vec<T, kVec> v = load<Vec<T, kVec>>((const T*)a.vol + L::plane(d0, e), lvo);
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) raw[e + j] = v.v[j];
+        for (int j = 0; j < kVec; ++j) raw.v[e + j] = v.v[j];
       } else if (left > 0) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) raw[e + j] = load<T>((const T*)a.vol + L::plane(d0, e), (Off)(lvo + (Off)min(j, left - 1) * (Off)sizeof(T)));
+        for (int j = 0; j < kVec; ++j)
+          raw.v[e + j] = load<T>((const T*)a.vol + L::plane(d0, e), (Off)(lvo + (Off)min(j, left - 1) * (Off)sizeof(T)));
       }
-      if (masked && left > 0) {
+      if (M != kNoMask && left > 0) {
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
-          seen[e + j] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], (Off)(lmo + (Off)min(j, left - 1) * (Off)a.ms[1]));
+          raw.seen[e + j] = load<uint8_t>(a.mask + L::plane(d0, e) * a.ms[1], (Off)(lmo + (Off)min(j, left - 1) * (Off)a.ms[1]));
       }
     }
+  }
+}
+template <MaskKind M, typename T, int G, int N>
+__device__ __forceinline__ void unpack_last(float (&x)[N], const Raw<T, N>& raw, int d0, int planes, int lane) {
+  using L = Spread<T, G>;
+  if (d0 + N * G <= planes) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool seen = M == kNoMask || (M == kMaskVectors ? (raw.word[e / 4] & (0xffu << e % 4 * 8)) != 0 : raw.seen[e] != 0);
+      x[e] = seen ? to_f32(raw.v[e]) : -INFINITY;
+    }
+  } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      x[e] = L::plane(d0, e) + lane * kVec < a.d && (!masked || seen[e]) ? to_f32(raw[e]) : -INFINITY;
+      x[e] = L::plane(d0, e) + lane * L::kVec < planes && (M == kNoMask || raw.seen[e]) ? to_f32(raw.v[e]) : -INFINITY;
   }
 }
 
@@ -444,8 +471,10 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   }
   Stats<K> st;
   for (int d0 = begin; d0 < end; d0 += kN) {
+    Raw<T, kN> raw;
+    load_first(raw, a, masked, d0, end, rvo, rmo);
     float x[kN];
-    read_first<T>(x, a, masked, d0, end, rvo, rmo);
+    unpack_first(x, raw, masked, d0, end);
     add_planes<1>(st, x, c, d0 + kN / 2 >= end, [&](int e) { return d0 + e; });
   }
   if constexpr (S > 1) {
@@ -472,7 +501,7 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
 }
 
 // Volume with the planes of a pixel next to each other (channels_last): four lanes per pixel, 8 planes per lane at a time.
-template <typename T, int K, typename Off>
+template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   constexpr int G = 4, N = 8;
   using L = Spread<T, G>;
@@ -483,13 +512,15 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q);
   const float c = a.scale * kLog2e;
-  const bool masked = a.mask && a.ms[1] != 0;
-  const uint8_t seen = a.mask && !masked ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
+  const uint8_t seen = M == kNoMask && a.mask ? load<uint8_t>(a.mask, mo) : 1;  // (used after the loop: nothing waits for it here)
   const int64_t given = a.plane ? load<int64_t>(a.plane, (Off)p * 8) : -1;
   Stats<K> st;
+  Raw<T, N> raw;
+  load_last<M, T, G>(raw, a, 0, lane, vo, mo);
   for (int d0 = 0; d0 < a.d; d0 += N * G) {
     float x[N];
-    read_last<T, G>(x, a, masked, d0, lane, vo, mo);
+    unpack_last<M, T, G>(x, raw, d0, a.d, lane);
+    if (d0 + N * G < a.d) load_last<M, T, G>(raw, a, d0 + N * G, lane, vo, mo);  // (under way during the arithmetic)
     st.template add<G>(x, c, [&](int e) { return L::plane(d0, e); });
   }
   st.s = group_sum<G>(st.s), st.t = group_sum<G>(st.t);
@@ -570,9 +601,11 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
   const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q), go = offset_of<Off>(a.gs, q) * (Off)sizeof(T);
   const bool masked = a.mask && a.ms[1] != 0;
   for (int d0 = blockIdx.y * kN; d0 < a.d; d0 += gridDim.y * kN) {
-    float x[kN];
-    read_first<T>(x, a, masked, d0, a.d, vo, mo);
+    Raw<T, kN> raw;
+    load_first(raw, a, masked, d0, a.d, vo, mo);
     const Pull<K, Off> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+    float x[kN];
+    unpack_first(x, raw, masked, d0, a.d);
     T* grad = (T*)((char*)a.grad + go);
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
@@ -583,23 +616,24 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
 }
 
 // the planes of a pixel next to each other, in the volume and in its gradient: four lanes per pixel, 16 bytes per lane, load and store
-template <typename T, int K, typename Off>
+template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
-  constexpr int G = 4;
+  constexpr int G = 4, N = 8;
   using L = Spread<T, G>;
   const int lane = threadIdx.x % G;
   const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q), go = offset_of<Off>(a.gs, q) * (Off)sizeof(T);
-  const bool masked = a.mask && a.ms[1] != 0;
-  float x[kN];
-  read_last<T, G>(x, a, masked, 0, lane, vo, mo);
-  Pull<K, Off> pull(a, p, q, a.mask && !masked && !load<uint8_t>(a.mask, mo));
+  Raw<T, N> raw;
+  load_last<M, T, G>(raw, a, 0, lane, vo, mo);
+  Pull<K, Off> pull(a, p, q, M == kNoMask && a.mask && !load<uint8_t>(a.mask, mo));
   pull.move(-lane * L::kVec);
   for (int d0 = 0;;) {
+    float x[N];
+    unpack_last<M, T, G>(x, raw, d0, a.d, lane);
 #pragma unroll
-    for (int e = 0; e < kN; e += L::kVec) {
+    for (int e = 0; e < N; e += L::kVec) {
       const int d = L::plane(d0, e) + lane * L::kVec;
       Vec<T, L::kVec> r;
 #pragma unroll
@@ -612,9 +646,9 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
           if (d + j < a.d) store((T*)a.grad + L::plane(d0, e) + j, (Off)(go + lane * 16u), r.v[j]);
       }
     }
-    d0 += kN * G;
+    d0 += N * G;
     if (d0 >= a.d) break;
-    read_last<T, G>(x, a, masked, d0, lane, vo, mo);
+    load_last<M, T, G>(raw, a, d0, lane, vo, mo);
   }
 }
 
@@ -649,6 +683,14 @@ void by_type(int dtype, F&& f) {
   else f(__hip_bfloat16{});
 }
 
+// the mask as the kernels with the planes innermost read it
+template <typename F>
+void by_mask(const uint8_t* mask, int64_t plane_stride, F&& f) {
+  if (!mask || plane_stride == 0) f(std::integral_constant<MaskKind, kNoMask>{});
+  else if (plane_stride == 1) f(std::integral_constant<MaskKind, kMaskVectors>{});
+  else f(std::integral_constant<MaskKind, kMaskBytes>{});
+}
+
 // lists of 0, 1, 4 and 8 slots
 template <typename F>
 void by_top(int top, F&& f) {
@@ -674,7 +716,8 @@ void launch_stats(const PlaneFwd& a, hipStream_t s) {
   //   D = 64:   76800 pixels 6.3 / 8.8 against 7.1 / 10.5; 307200 pixels 15.5 / 23.4 against 16.8 / 20.8
   //   D = 128: 153600 pixels 15.3 / 20.0 against 15.6 / 22.2; 307200 pixels 32.8 / 40.6 against 33.0 / 37.3
   const bool share = (int64_t)pixels < 2400 * ((int64_t)a.d - 24);
-  if (a.vs[1] == 1) DT_LAUNCH((plane_stats_last_kernel<T, K, uint32_t>), by_four, block, 0, s, a);
+  if (a.vs[1] == 1)
+    by_mask(a.mask, a.ms[1], [&](auto m) { DT_LAUNCH((plane_stats_last_kernel<T, K, m.value, uint32_t>), by_four, block, 0, s, a); });
   else if (share) DT_LAUNCH((plane_stats_first_kernel<T, K, 4, uint32_t>), by_four, block, 0, s, a);
   else DT_LAUNCH((plane_stats_first_kernel<T, K, 1, uint32_t>), by_pixel, block, 0, s, a);
 }
@@ -682,7 +725,8 @@ void launch_stats(const PlaneFwd& a, hipStream_t s) {
 template <typename T>
 void launch_stats_wide(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  if (a.vs[1] == 1) DT_LAUNCH((plane_stats_last_kernel<T, 8, int64_t>), dim3((pixels + 63) / 64), dim3(256), 0, s, a);
+  if (a.vs[1] == 1)
+    by_mask(a.mask, a.ms[1], [&](auto m) { DT_LAUNCH((plane_stats_last_kernel<T, 8, m.value, int64_t>), dim3((pixels + 63) / 64), dim3(256), 0, s, a); });
   else DT_LAUNCH((plane_stats_first_kernel<T, 8, 1, int64_t>), dim3((pixels + 255) / 256), dim3(256), 0, s, a);
 }
 
@@ -690,8 +734,13 @@ template <typename T, int K, typename Off>
 void launch_grad(const PlaneBwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
   const dim3 block(256), by_four((pixels + 63) / 64), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + kN - 1) / kN));
-  if (a.vs[1] == 1 && a.gs[1] == 1) DT_LAUNCH((plane_grad_last_kernel<T, K, Off>), by_four, block, 0, s, a);
-  else DT_LAUNCH((plane_grad_first_kernel<T, K, Off>), by_pixel, block, 0, s, a);
+  if (a.vs[1] == 1 && a.gs[1] == 1) {
+    // (bytes also where they lie next to each other: the vectors cost this kernel twice the registers)
+    if (a.mask && a.ms[1] != 0) DT_LAUNCH((plane_grad_last_kernel<T, K, kMaskBytes, Off>), by_four, block, 0, s, a);
+    else DT_LAUNCH((plane_grad_last_kernel<T, K, kNoMask, Off>), by_four, block, 0, s, a);
+  } else {
+    DT_LAUNCH((plane_grad_first_kernel<T, K, Off>), by_pixel, block, 0, s, a);
+  }
 }
 
 int check_desc(const char* what, const dt_plane_desc* d) {
