@@ -448,6 +448,9 @@ __device__ __forceinline__ void add_planes(Stats<K>& st, const float (&x)[kN], f
 // Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel.
 // S = 4: the four waves of a workgroup share 64 pixels, a quarter of the planes each; the partial results change places through LDS so
 // that four neighbouring lanes hold the four parts of a pixel, and all waves join and write 16 pixels each.
+// Bound: memory in float32 (16 x 64 x 120 x 160 pixels, 4 alternatives: 21.3 us, 4.7 TB/s of what has to move; a large copy on this card
+// reaches 4.8) and in float16 without alternatives (8 x 128 x 240 x 320: 36.6 us, 4.6 TB/s); vector instructions in float16 with
+// alternatives (16 x 64 x 120 x 160, 4 of them: 19.1 us, 3.1 TB/s); latency below about 50000 pixels (one keyframe 3.5 to 4.7 us).
 template <typename T, int K, int S, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -500,7 +503,11 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   if (at < pixels) write<K, S, Off>(a, p, q, st, given, x_given, group);
 }
 
-// Volume with the planes of a pixel next to each other (channels_last): four lanes per pixel, 8 planes per lane at a time.
+// Volume with the planes of a pixel next to each other (channels_last): four lanes per pixel, 8 planes per lane at a time.  Two loads of
+// a lane cover the halves of a 128-byte line, so four lanes fetch whole lines; 16 lanes per pixel paid more for joining and writing
+// (8 x 64 x 120 x 160, 4 alternatives, an early version: 55 us against 19), two lanes and 16 planes at a time were within 10 % either way.
+// Bound: memory from about 64 float32 planes on (16 x 64 x 120 x 160, 4 alternatives: 20.7 us, 4.8 TB/s), the vector instructions of
+// joining and writing a pixel below (8 x 32 x 120 x 160: 9.3 us, 3.2 TB/s) and in 16 bits; latency at one keyframe (3.1 to 4.2 us).
 template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   constexpr int G = 4, N = 8;
@@ -593,6 +600,7 @@ struct Pull {
 };
 
 // neighbouring pixels next to each other: one lane per pixel and 16 planes, blockIdx.y numbers the groups of planes
+// Bound: memory (float16, 16 x 64 x 96 x 128: 13.4 us, 4.1 TB/s with the pixels' statistics read once per 16 planes)
 template <typename T, int K, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
   const uint32_t p = blockIdx.x * 256u + threadIdx.x;
@@ -616,6 +624,7 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
 }
 
 // the planes of a pixel next to each other, in the volume and in its gradient: four lanes per pixel, 16 bytes per lane, load and store
+// Bound: memory (4 x 256 x 120 x 160, mask, 4 alternatives: 37.8 us, 4.8 TB/s)
 template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
   constexpr int G = 4, N = 8;
@@ -654,7 +663,8 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
 
 // ---- planes of depths ------------------------------------------------------------------------------------------------------------
 // 64-bit differences of 32-bit depths are exact wherever two of them are close, so a tie is a tie; 16 planes' loads are in flight together.
-// Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 5.1 us with four).
+// Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 4.6 us, 5.1 with four waves).
+// Bound: memory where planes vary over the image (8 x 96 x 240 x 320: 46 us, 5.2 TB/s, a part from the last-level cache), else latency.
 __global__ void __launch_bounds__(64) nearest_planes_kernel(PlaneNear a) {
   const uint32_t p = blockIdx.x * 64u + threadIdx.x;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
@@ -712,9 +722,9 @@ void launch_stats(const PlaneFwd& a, hipStream_t s) {
   const dim3 block(256), by_pixel((pixels + 255) / 256), by_four((pixels + 63) / 64);
   // Four waves per 64 pixels pay (the exchange, four lanes writing a pixel) where few pixels with many planes would leave the chip idle.
   // Measured us, fp32, 0 / 4 alternatives, four waves against one:
-  //   D = 16:   19200 pixels 3.5 / 4.4 against 2.8 / 3.6;  307200 pixels 13.0 / 19.1 against  6.3 /  9.4
-  //   D = 64:   76800 pixels 6.3 / 8.8 against 7.1 / 10.5; 307200 pixels 15.5 / 23.4 against 16.8 / 20.8
-  //   D = 128: 153600 pixels 15.3 / 20.0 against 15.6 / 22.2; 307200 pixels 32.8 / 40.6 against 33.0 / 37.3
+  //   D = 16:   19200 pixels  3.6 /  4.3 against  2.8 /  3.5; 307200 pixels 13.0 / 18.5 against  6.4 /  9.2
+  //   D = 64:   76800 pixels  6.3 /  8.7 against  7.1 / 10.5; 307200 pixels 15.5 / 22.7 against 17.0 / 21.1
+  //   D = 128: 153600 pixels 15.4 / 20.0 against 15.5 / 23.2; 307200 pixels 32.9 / 39.4 against 32.9 / 36.7
   const bool share = (int64_t)pixels < 2400 * ((int64_t)a.d - 24);
   if (a.vs[1] == 1)
     by_mask(a.mask, a.ms[1], [&](auto m) { DT_LAUNCH((plane_stats_last_kernel<T, K, m.value, uint32_t>), by_four, block, 0, s, a); });

@@ -249,7 +249,7 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
                                void* grad_volume, dt_stream_t s);
 /* The plane a metric depth falls on: argmin_d |depth - planes_d| per pixel (differences in 64 bits: exact), the lowest plane of
  * equal ones; -1 where the depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x;
- * 0 along a broadcast axis); a NaN plane is never the nearest. */
+ * 0 along a broadcast axis, none negative); a plane that is no finite number is never the nearest. */
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
                              int w, int64_t* plane_bhw, dt_stream_t s);
 

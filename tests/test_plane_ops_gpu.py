@@ -124,6 +124,33 @@ def test_views(dtype):
             raise AssertionError(f"{name}: {e}") from e
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [3, 8, 31, 32, 33, 64, 77, 130])
+def test_mask_layouts(D, dtype):
+    """Every layout of a mask with every layout of the volume: bytes of neighbouring planes next to each other (any alignment), far
+    apart, on another axis, shared by pixels or batch elements."""
+    g = torch.Generator().manual_seed(D)
+    b, h, w = 2, 5, 9
+    full = torch.rand(b, D, h, w, generator=g) > 0.4
+    full[0, :, 2, 3] = False
+    flat = torch.zeros(3 + full.numel(), dtype=torch.bool, device=DEV)
+    odd = flat[3:].view(b, h, w, D).permute(0, 3, 1, 2)
+    odd.copy_(full)
+    masks = {"planes far apart": full.to(DEV), "planes innermost": full.to(DEV).contiguous(memory_format=torch.channels_last),
+             "planes innermost, three bytes off": odd, "planes second": full.permute(0, 2, 1, 3).contiguous().to(DEV).permute(0, 2, 1, 3),
+             "one row for all pixels": full[:1, :, :1, :1].to(DEV), "one per pixel": full[:, :1].to(DEV),
+             "one for all": full[:1, 1:2, :1, :1].to(DEV)}
+    for layout in ("last", "first"):
+        vol, _, plane, _ = make((b, D, h, w), dtype, layout, seed=3)
+        for name, m in masks.items():
+            try:
+                r = plane_ops.plane_log_probs(vol, plane, top=min(3, D), mask_bdhw=m)
+                ref.check_stats(r, vol, plane, min(3, D), 1.0, m)
+                _check_grad(vol, plane, min(2, D), 1.0, m, seed=8)
+            except AssertionError as e:
+                raise AssertionError(f"{layout}, {name}: {e}") from e
+
+
 def _check_grad(vol, plane, top, scale, mask, seed=0, use=("lp", "ent", "lsum", "top"), size=1.0):
     g = torch.Generator().manual_seed(100 + seed)
     b, D, h, w = vol.shape
@@ -339,9 +366,13 @@ def test_indices_beyond_32_bits():
     mask = marks.as_strided((1, 5, 4, 8), (0, far, 8, 1))
     mask.copy_(torch.rand(1, 5, 4, 8, generator=g) > 0.3)
     plane = torch.randint(-1, 5, (1, 4, 8), generator=g).to(DEV)
-    r = plane_ops.plane_log_probs(vol, plane, top=4, mask_bdhw=mask)
-    ref.check_stats(r, vol.contiguous(), plane, 4, 1.0, mask.contiguous())
-    del marks, mask
+    planes = torch.empty(4 * far + 64, dtype=F32, device=DEV).as_strided((1, 5, 4, 8), (0, far, 8, 1))   # 23 GB
+    planes.copy_(torch.rand(1, 5, 4, 8, generator=g) + 0.25)
+    r = plane_ops.plane_log_probs(vol, plane, top=4, mask_bdhw=mask, depth_planes_bdhw=planes)
+    ref.check_stats(r, vol.contiguous(), plane, 4, 1.0, mask.contiguous(), planes.contiguous())
+    dep = torch.rand(1, 4, 8, generator=g).to(DEV) * 1.5
+    assert torch.equal(plane_ops.nearest_planes(dep, planes).cpu(), ref.nearest(dep, planes.contiguous()))
+    del marks, mask, planes
     # planes next to each other, pixels far apart
     vol = store.as_strided((1, 16, 1, 5), (0, 1, 0, far))
     vol.copy_(torch.randn(1, 16, 1, 5, generator=g))
