@@ -372,13 +372,19 @@ def test_indices_beyond_32_bits():
     ref.check_stats(r, vol.contiguous(), plane, 4, 1.0, mask.contiguous(), planes.contiguous())
     dep = torch.rand(1, 4, 8, generator=g).to(DEV) * 1.5
     assert torch.equal(plane_ops.nearest_planes(dep, planes).cpu(), ref.nearest(dep, planes.contiguous()))
-    del marks, mask, planes
-    # planes next to each other, pixels far apart
-    vol = store.as_strided((1, 16, 1, 5), (0, 1, 0, far))
+    _check_grad(vol, plane, 2, 1.0, mask, seed=1)
+    del mask, planes
+    # planes next to each other, pixels far apart: no mask, mask bytes like the scores, a mask far apart in planes
+    vol = store.as_strided((1, 16, 1, 5), (0, 1, 0, far - 8))
     vol.copy_(torch.randn(1, 16, 1, 5, generator=g))
-    r = plane_ops.plane_log_probs(vol, top=4)
-    ref.check_stats(r, vol.contiguous(), top=4)
-    del store, vol
+    like = marks.as_strided((1, 16, 1, 5), (0, 1, 0, far - 8))
+    like.copy_(torch.rand(1, 16, 1, 5, generator=g) > 0.3)
+    plane = torch.randint(-1, 16, (1, 1, 5), generator=g).to(DEV)
+    for m in (None, like, like.contiguous()):
+        r = plane_ops.plane_log_probs(vol, plane, top=4, mask_bdhw=m)
+        ref.check_stats(r, vol.contiguous(), plane, 4, 1.0, m.contiguous() if m is not None else None)
+        _check_grad(vol, plane, 4, 1.0, m, seed=2)
+    del store, marks, vol, like, m
     # a dense gradient of more than 2^32 bytes and 2^31 elements: the far end of a real volume
     big = torch.empty(1, 16, 11586, 11586, dtype=F16, device=DEV).fill_(-1.0)
     assert big.numel() > 1 << 31
@@ -395,6 +401,46 @@ def test_indices_beyond_32_bits():
     want, err = ref.gradient(tail, None, 0, 1.0, None, g_lsum=torch.ones(1, 1, 40))
     ref.close(cut(grad), want, err * 1.01 + HALF_STEP[F16] * want.abs() + TINY[F16])
     assert bool((grad[:, :, :-1] == 0.0625).all())
+
+
+@pytest.mark.parametrize("layout,D", [("first", 1), ("last", 2)])
+def test_more_pixels_than_32_bit_output_offsets(layout, D):
+    """538 million pixels: the alternatives' planes alone are 4.3 GB."""
+    n = 23200
+    g = torch.Generator().manual_seed(D)
+    vol = torch.empty((1, D, n, n), dtype=F16, device=DEV,
+                      memory_format=torch.channels_last if layout == "last" else torch.contiguous_format).zero_()
+    tail = torch.randn(1, D, 1, 50, generator=g).to(F16).to(DEV)
+    vol[:, :, -1:, -50:] = tail
+    plane = torch.zeros(1, n, n, dtype=torch.int64, device=DEV)
+    plane[0, -1, -50:] = D - 1
+    vol.requires_grad_(True)
+    r = plane_ops.plane_log_probs(vol, plane, top=1)
+    cut = lambda t: t[..., -1:, -50:]
+    want = ref.stats(tail, torch.full((1, 1, 50), D - 1), 1)
+    ref.close(cut(r.log_prob_bhw), want["log_prob"], ref.bound_a(D), 4 * ref.U)
+    ref.close(cut(r.entropy_bhw), want["entropy"], ref.bound_b(D))
+    assert torch.equal(cut(r.top_plane_bkhw).cpu(), want["top_plane"])
+    assert int(r.top_plane_bkhw[:, :, :-1].abs().max()) == 0
+    assert abs(float(r.entropy_bhw[0, 0, 0]) - math.log(D)) <= ref.bound_b(D) and bool((r.entropy_bhw[0, :-1] == r.entropy_bhw[0, 0, 0]).all())
+    grad, = torch.autograd.grad(r.log_prob_bhw, vol, torch.ones_like(r.entropy_bhw))
+    wg, err = ref.gradient(tail, torch.full((1, 1, 50), D - 1), 0, 1.0, None, g_lp=torch.ones(1, 1, 50))
+    ref.close(cut(grad), wg, err * 1.01 + HALF_STEP[F16] * wg.abs() + TINY[F16])
+    assert bool((grad[0, 0, :-1] == (0.0 if D == 1 else 0.5)).all())
+
+
+def test_garbage_in_masked_pixels():
+    """A mask of one flag per pixel: nothing of a hidden pixel's scores reaches an output, on either layout."""
+    for layout in ("last", "first"):
+        for shape in ((2, 40, 6, 7), (1, 8, 30, 40)):
+            vol, m, plane, _ = make(shape, layout=layout, mask="pixel", seed=90)
+            bad = torch.where(m, vol, torch.full_like(vol, math.nan))
+            bad[:, 1::3] = torch.where(m, bad[:, 1::3], torch.full_like(bad[:, 1::3], math.inf))
+            a = plane_ops.plane_log_probs(vol, plane, top=4, mask_bdhw=m)
+            b = plane_ops.plane_log_probs(bad.contiguous(memory_format=torch.channels_last if layout == "last" else torch.contiguous_format),
+                                          plane, top=4, mask_bdhw=m)
+            assert all((x is None and y is None) or torch.equal(x, y) for x, y in zip(a, b))
+            _check_grad(bad, plane, 4, 1.0, m, seed=4)
 
 
 @pytest.mark.parametrize("shape", [(1, 64, 12, 16), (2, 33, 7, 5)], ids=str)
