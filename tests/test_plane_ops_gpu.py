@@ -59,6 +59,28 @@ def test_stats(shape, dtype, layout):
             assert (a is None and b is None) or torch.equal(a, b)
 
 
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("shape", [(1, 9, 3, 70), (2, 24, 5, 13), (1, 20, 6, 41), (2, 64, 5, 13), (1, 100, 4, 9)], ids=str)
+def test_every_number_of_alternatives(shape, layout):
+    for top in range(9):
+        vol, m, plane, planes = make(shape, F32, layout, "plane", seed=30 + top)
+        planes = planes if top else None
+        r = plane_ops.plane_log_probs(vol, plane, top=top, mask_bdhw=m, depth_planes_bdhw=planes)
+        ref.check_stats(r, vol, plane, top, 1.0, m, planes)
+        _check_grad(vol, plane, top, 1.0, m, seed=top, use=("lp", "ent", "lsum") + (("top",) if top else ()))
+
+
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("shape,dtype,mask,top", [((1, 40, 200, 210), F32, "plane", 3), ((3, 64, 180, 185), F16, "pixel", 5),
+                                                  ((2, 33, 121, 163), BF16, "none", 1)], ids=["40", "64", "33"])
+def test_many_pixels(shape, dtype, mask, top, layout):
+    """Enough pixels that a lane goes through all planes of its pixel by itself (pixels innermost), several chunks of them."""
+    vol, m, plane, planes = make(shape, dtype, layout, mask, seed=12)
+    r = plane_ops.plane_log_probs(vol, plane, top=top, scale=0.5, mask_bdhw=m, depth_planes_bdhw=planes)
+    ref.check_stats(r, vol, plane, top, 0.5, m, planes)
+    _check_grad(vol, plane, top, 0.5, m, seed=13)
+
+
 def test_optional_inputs():
     vol, m, plane, planes = make((2, 20, 5, 7))
     r = plane_ops.plane_log_probs(vol)
@@ -422,7 +444,7 @@ def test_more_pixels_than_32_bit_output_offsets(layout, D):
     ref.close(cut(r.entropy_bhw), want["entropy"], ref.bound_b(D))
     assert torch.equal(cut(r.top_plane_bkhw).cpu(), want["top_plane"])
     assert int(r.top_plane_bkhw[:, :, :-1].abs().max()) == 0
-    assert abs(float(r.entropy_bhw[0, 0, 0]) - math.log(D)) <= ref.bound_b(D) and bool((r.entropy_bhw[0, :-1] == r.entropy_bhw[0, 0, 0]).all())
+    assert abs(float(r.entropy_bhw.detach()[0, 0, 0]) - math.log(D)) <= ref.bound_b(D) and bool((r.entropy_bhw[0, :-1] == r.entropy_bhw[0, 0, 0]).all())
     grad, = torch.autograd.grad(r.log_prob_bhw, vol, torch.ones_like(r.entropy_bhw))
     wg, err = ref.gradient(tail, torch.full((1, 1, 50), D - 1), 0, 1.0, None, g_lp=torch.ones(1, 1, 50))
     ref.close(cut(grad), wg, err * 1.01 + HALF_STEP[F16] * wg.abs() + TINY[F16])
