@@ -483,7 +483,11 @@ class _HotPathDepthModel(nn.Module):
                   return_mask=return_mask)
         if isinstance(self.cost_volume, FeatureMeshHintVolumeManager):  # the other managers take no hints
             kw["cv_depth_hint_dict"] = cv_depth_hint_dict
-        cost_volume, lowest_cost, planes, overall_mask = self.cost_volume(**kw)
+        statistics = getattr(self, "_plane_statistics", None) is not None
+        if statistics:  # (volume_stage keeps the planes to itself)
+            cost_volume, lowest_cost, planes, overall_mask = self.cost_volume(**kw)
+        else:
+            cost_volume, lowest_cost, overall_mask = self.volume_stage(kw)
         # graph mode: the replay is split here so that the hook below runs between the halves -- only when a hook is
         # waiting at capture time (every cut is one more hipGraphLaunch per replay)
         if "after_volume" in self.__dict__ or _graphs.recording():
@@ -495,7 +499,7 @@ class _HotPathDepthModel(nn.Module):
             # loops.matching_lookahead encodes the next frame's keyframe here
             hook()
         outputs = self.network_stage(cur_feats, cost_volume, lowest_cost, overall_mask)
-        if getattr(self, "_plane_statistics", None) is not None:
+        if statistics:
             self._add_plane_statistics(outputs, cost_volume, planes)
         return outputs
 
