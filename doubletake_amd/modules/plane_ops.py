@@ -105,8 +105,21 @@ def _dense_f32(g):
     return g.to(torch.float32).contiguous()
 
 
+def _check_saved(ctx, vol, plane, mask, ent, tpl):
+    """Hooks on saved tensors may bring a tensor back in another layout than it was saved in, which is fine, but also on another device
+    or of another type or size, and the kernel is given addresses: refused here."""
+    dev, (b, _, h, w) = ctx.rows.device, ctx.shape
+    for name, t, dtype, shape in (("volume_bdhw", vol, ctx.dtype, ctx.shape), ("plane_bhw", plane, torch.int64, (b, h, w)),
+                                  ("mask_bdhw", mask, torch.bool, ctx.shape), ("entropy_bhw", ent, torch.float32, (b, h, w)),
+                                  ("top_plane_bkhw", tpl, torch.int64, (b, ctx.top, h, w))):
+        if t is not None and (t.dtype is not dtype or t.shape != shape or t.device != dev):
+            raise RuntimeError(f"{name} was saved as {dtype} {tuple(shape)} on {dev}; a hook on saved tensors brought it back as "
+                               f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
     vol, plane, mask, ent, tpl = ctx.saved_tensors
+    _check_saved(ctx, vol, plane, mask, ent, tpl)
     g_lp, g_ent, g_lsum, g_top = _dense_f32(g_lp), _dense_f32(g_ent), _dense_f32(g_lsum), _dense_f32(g_top)
     grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
     n = ent.numel()
@@ -132,6 +145,7 @@ class _PlaneLogProbsFn(torch.autograd.Function):
         # made here, neither inputs nor outputs.  The engine runs a backward on the stream its forward ran on: the handle is kept, asking
         # for it in the engine's thread costs 6 us
         ctx.rows, ctx.stream, ctx.top, ctx.scale = rows, stream, top, scale
+        ctx.dtype, ctx.shape = vol.dtype, vol.shape
         return tuple(out)
 
     @staticmethod

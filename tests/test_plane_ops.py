@@ -2,6 +2,7 @@
 against torch's log_softmax and against differences."""
 import ctypes as C
 import math
+import types
 
 import pytest
 import torch
@@ -186,3 +187,40 @@ def test_model_refuses_bad_statistics_settings_and_loops_need_them():
     got = loops._depth_for_fusion({"depth_pred_s0_b1hw": depth, "plane_log_prob_bhw": lp}, None, min_plane_log_prob=-1.0)
     want = torch.tensor([[1.0, -1, -1], [1, 1, -1]]).repeat_interleave(2, 0).repeat_interleave(2, 1)
     assert torch.equal(got[0, 0], want) and bool((depth == 1).all())
+
+
+def _saved(**kw):
+    """What a backward pass of a [2, 5, 3, 4] volume with a mask, given planes and two alternatives finds saved."""
+    b, D, h, w, top = 2, 5, 3, 4, 2
+    t = dict(vol=torch.zeros(b, D, h, w), plane=torch.zeros(b, h, w, dtype=torch.int64), mask=torch.ones(b, D, h, w, dtype=torch.bool),
+             ent=torch.zeros(b, h, w), tpl=torch.zeros(b, top, h, w, dtype=torch.int64))
+    ctx = types.SimpleNamespace(rows=torch.zeros(2, b, h, w), stream=None, top=top, scale=1.0, dtype=torch.float32,
+                                shape=t["vol"].shape)
+    t.update(kw)
+    ctx.saved_tensors = tuple(t.values())
+    return ctx
+
+
+@pytest.mark.parametrize("name,bring", [
+    ("vol", lambda t: t.half()), ("vol", lambda t: t[:, :4]), ("vol", lambda t: t.to("meta")),
+    ("plane", lambda t: t.int()), ("plane", lambda t: t.to("meta")), ("plane", lambda t: t[:1]),
+    ("mask", lambda t: t.float()), ("mask", lambda t: t[:, :1]), ("mask", lambda t: t.to("meta")),
+    ("ent", lambda t: t.half()), ("ent", lambda t: t[0]), ("tpl", lambda t: t.int()), ("tpl", lambda t: t[:, :1])])
+def test_backward_refuses_saved_tensors_brought_back_as_others(name, bring, monkeypatch):
+    """A hook on saved tensors returned another device, type or size: refused before the kernel is given an address."""
+    calls = []
+
+    class Lib:
+        def dt_cv_plane_log_probs_grad(self, *a):
+            calls.append(a)
+            return 0
+
+    monkeypatch.setattr(_abi, "lib", Lib)
+    g = torch.ones(2, 3, 4)
+    good = _saved()
+    assert plane_ops._backward(good, g, g, g, torch.ones(2, 2, 3, 4), None, None)[0].shape == good.shape and len(calls) == 1
+    order = ("vol", "plane", "mask", "ent", "tpl")
+    bad = _saved(**{name: bring(good.saved_tensors[order.index(name)])})
+    with pytest.raises(RuntimeError, match="hook on saved tensors"):
+        plane_ops._backward(bad, g, g, g, torch.ones(2, 2, 3, 4), None, None)
+    assert len(calls) == 1

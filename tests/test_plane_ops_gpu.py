@@ -552,3 +552,14 @@ def test_depth_map_to_log_probability():
     r = plane_ops.plane_log_probs(vol, idx, top=2, depth_planes_bdhw=planes)
     assert torch.equal(r.log_prob_bhw, r.top_log_prob_bkhw[:, 0])
     assert torch.equal(r.top_plane_bkhw[:, :1], first.top_plane_bkhw)
+
+
+@pytest.mark.parametrize("pack", [lambda t: t.cpu(), lambda t: t.half() if t.dtype == F32 else t, lambda t: t[..., :1]],
+                         ids=["host", "half", "sliced"])
+def test_saved_tensors_brought_back_as_others_are_refused(pack):
+    vol, m, plane, _ = make((2, 20, 9, 11), mask="plane", seed=47)
+    leaf = vol.detach().requires_grad_(True)
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        r = plane_ops.plane_log_probs(leaf, plane, top=2, mask_bdhw=m)
+    with pytest.raises(RuntimeError, match="hook on saved tensors"):
+        r.entropy_bhw.sum().backward()
