@@ -33,6 +33,7 @@ struct PlaneFwd {
   int b, d, h, w, top;
   float scale;
   Div by_hw, by_w;
+  uint32_t first;  // pixel the launch begins at (by_range; 0 with 32-bit offsets)
 };
 DT_ARG_POINTERS(PlaneFwd, offsetof(PlaneFwd, vol), offsetof(PlaneFwd, mask), offsetof(PlaneFwd, plane), offsetof(PlaneFwd, planes),
                 offsetof(PlaneFwd, log_prob), offsetof(PlaneFwd, entropy), offsetof(PlaneFwd, log_sum),
@@ -51,6 +52,7 @@ struct PlaneBwd {
   int b, d, h, w, top;
   float scale;
   Div by_hw, by_w;
+  uint32_t first;  // as PlaneFwd's
 };
 DT_ARG_POINTERS(PlaneBwd, offsetof(PlaneBwd, vol), offsetof(PlaneBwd, mask), offsetof(PlaneBwd, plane), offsetof(PlaneBwd, entropy),
                 offsetof(PlaneBwd, top_plane), offsetof(PlaneBwd, row_max), offsetof(PlaneBwd, row_log),
@@ -95,6 +97,13 @@ __device__ __forceinline__ Pixel pixel_of(uint32_t p, int h, int w, Div by_hw, D
 template <typename Off>
 __device__ __forceinline__ Off offset_of(const int64_t (&s)[4], const Pixel& q) {
   return (Off)q.b * (Off)s[0] + (Off)q.y * (Off)s[2] + (Off)q.x * (Off)s[3];
+}
+
+// the pixel this quad of lanes works on
+template <typename Off, typename A>
+__device__ __forceinline__ uint32_t quad_pixel(const A& a) {
+  const uint32_t at = blockIdx.x * 64u + threadIdx.x / 4;
+  return sizeof(Off) == 8 ? a.first + at : at;
 }
 
 // A launch-uniform 64-bit base plus an offset in bytes per lane.  The empty statement keeps the base in scalar registers: left to itself
@@ -513,7 +522,7 @@ __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   constexpr int G = 4, N = 8;
   using L = Spread<T, G>;
   const int lane = threadIdx.x % G;
-  const uint32_t at = blockIdx.x * (256u / G) + threadIdx.x / G;
+  const uint32_t at = quad_pixel<Off>(a);
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
   const uint32_t p = min(at, pixels - 1);
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
@@ -630,7 +639,7 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
   constexpr int G = 4, N = 8;
   using L = Spread<T, G>;
   const int lane = threadIdx.x % G;
-  const uint32_t p = blockIdx.x * (256u / G) + threadIdx.x / G;
+  const uint32_t p = quad_pixel<Off>(a);
   if (p >= (uint32_t)a.b * a.h * a.w) return;
   const Pixel q = pixel_of(p, a.h, a.w, a.by_hw, a.by_w);
   const Off vo = offset_of<Off>(a.vs, q) * (Off)sizeof(T), mo = offset_of<Off>(a.ms, q), go = offset_of<Off>(a.gs, q) * (Off)sizeof(T);
@@ -716,6 +725,15 @@ int64_t span_of(const int64_t (&s)[4], int b, int h, int w, int64_t planes, int 
 }
 constexpr int64_t kNear = (int64_t)1 << 32;
 
+// Four lanes per pixel, in launches of at most 2^29 pixels: from 2^30 on a single one would have 2^32 work items, more than a grid takes.
+// (With 32-bit offsets a volume has fewer than 2^29 pixels, kNear / 8.)
+template <typename A, typename F>
+void by_range(A a, F&& launch) {
+  constexpr uint32_t kRange = 1u << 29;
+  const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
+  for (a.first = 0; a.first < pixels; a.first += kRange) launch(a, dim3((std::min(pixels - a.first, kRange) + 63) / 64));
+}
+
 template <typename T, int K>
 void launch_stats(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
@@ -736,18 +754,22 @@ template <typename T>
 void launch_stats_wide(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
   if (a.vs[1] == 1)
-    by_mask(a.mask, a.ms[1], [&](auto m) { DT_LAUNCH((plane_stats_last_kernel<T, 8, m.value, int64_t>), dim3((pixels + 63) / 64), dim3(256), 0, s, a); });
+    by_mask(a.mask, a.ms[1], [&](auto m) {
+      by_range(a, [&](const PlaneFwd& r, dim3 grid) { DT_LAUNCH((plane_stats_last_kernel<T, 8, m.value, int64_t>), grid, dim3(256), 0, s, r); });
+    });
   else DT_LAUNCH((plane_stats_first_kernel<T, 8, 1, int64_t>), dim3((pixels + 255) / 256), dim3(256), 0, s, a);
 }
 
 template <typename T, int K, typename Off>
 void launch_grad(const PlaneBwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
-  const dim3 block(256), by_four((pixels + 63) / 64), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + kN - 1) / kN));
+  const dim3 block(256), by_pixel((pixels + 255) / 256, std::min(65535, (a.d + kN - 1) / kN));
   if (a.vs[1] == 1 && a.gs[1] == 1) {
-    // (bytes also where they lie next to each other: the vectors cost this kernel twice the registers)
-    if (a.mask && a.ms[1] != 0) DT_LAUNCH((plane_grad_last_kernel<T, K, kMaskBytes, Off>), by_four, block, 0, s, a);
-    else DT_LAUNCH((plane_grad_last_kernel<T, K, kNoMask, Off>), by_four, block, 0, s, a);
+    by_range(a, [&](const PlaneBwd& r, dim3 grid) {
+      // (bytes also where they lie next to each other: the vectors cost this kernel twice the registers)
+      if (a.mask && a.ms[1] != 0) DT_LAUNCH((plane_grad_last_kernel<T, K, kMaskBytes, Off>), grid, block, 0, s, r);
+      else DT_LAUNCH((plane_grad_last_kernel<T, K, kNoMask, Off>), grid, block, 0, s, r);
+    });
   } else {
     DT_LAUNCH((plane_grad_first_kernel<T, K, Off>), by_pixel, block, 0, s, a);
   }

@@ -174,7 +174,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
 
     Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice): the gradient has the volume's
     type and layout.  A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on
-    the current stream and can be captured into a graph; capture a backward pass only together with its forward pass."""
+    the current stream (planes innermost: one per 2^29 pixels) and can be captured into a graph; capture a backward pass only together with its forward pass."""
     vol = volume_bdhw
     if vol.dim() != 4:
         raise ValueError(f"volume_bdhw must be [b, D, h, w], got {tuple(vol.shape)}")

@@ -563,3 +563,31 @@ def test_saved_tensors_brought_back_as_others_are_refused(pack):
         r = plane_ops.plane_log_probs(leaf, plane, top=2, mask_bdhw=m)
     with pytest.raises(RuntimeError, match="hook on saved tensors"):
         r.entropy_bhw.sum().backward()
+
+
+def test_more_channels_last_pixels_than_one_grid_takes():
+    """2^30 pixels and some: four lanes each are more than 2^32 work items.  Pixels at both ends and around every 2^29th."""
+    h, w, D = 32768, 32800, 2
+    assert h * w > 1 << 30
+    g = torch.Generator().manual_seed(3)
+    vol = torch.empty((1, D, h, w), dtype=F16, device=DEV, memory_format=torch.channels_last).zero_()
+    rows = vol.permute(0, 2, 3, 1).reshape(h * w, D)   # (a view: planes are innermost)
+    at = torch.cat([torch.arange(n - 40, n + 40) for n in (40, 1 << 28, 1 << 29, 3 << 28, 1 << 30, h * w - 40)]).to(DEV)
+    part = torch.randn(len(at), D, generator=g).to(F16)
+    rows[at] = part.to(DEV)
+    tail = part.T.reshape(1, D, 1, -1)
+    want = ref.stats(tail)
+    ref.close(plane_ops.plane_log_probs(vol).entropy_bhw.view(-1)[at], want["entropy"].view(-1), ref.bound_b(D))
+    mask = torch.ones(1, 1, 1, 1, dtype=torch.bool, device=DEV).expand(1, D, 1, 1)
+    vol.requires_grad_(True)
+    r = plane_ops.plane_log_probs(vol, mask_bdhw=mask)
+    ref.close(r.log_sum_bhw.view(-1)[at], want["log_sum"].view(-1), ref.bound_a(D) + 4 * ref.U * 8)
+    for a, e in ((0, at[80]), (at[159] + 1, at[160]), (at[399] + 1, at[400])):   # what lies between them: equal scores
+        assert bool((r.entropy_bhw.view(-1)[a + 80:e] == r.entropy_bhw.view(-1)[1 << 27]).all())
+    assert abs(float(r.entropy_bhw.detach().view(-1)[1 << 27]) - math.log(2)) <= ref.bound_b(2)
+    grad, = torch.autograd.grad(r.log_sum_bhw, vol, torch.ones_like(r.log_sum_bhw))
+    got = grad.permute(0, 2, 3, 1).reshape(h * w, D)
+    wg, err = ref.gradient(tail, None, 0, 1.0, None, g_lsum=torch.ones(1, 1, len(at)))
+    ref.close(got[at], wg[0, :, 0].T, (err * 1.01 + HALF_STEP[F16] * wg.abs() + TINY[F16])[0, :, 0].T)
+    for a, e in ((0, at[80]), (at[159] + 1, at[160]), (at[399] + 1, at[400])):
+        assert bool((got[a + 80:e] == 0.5).all())
