@@ -219,6 +219,8 @@ __device__ __forceinline__ void merge_lanes(double (&k)[K]) {
 // m: largest score so far (-inf: none); with y = c (x - m), c = scale log2 e: s = sum 2^y and t = sum 2^y y.  When the maximum moves
 // by delta = c (m_old - m_new): s' = s 2^delta, t' = (t + delta s) 2^delta.  A NaN score, or +inf (inf - inf), makes s and with it
 // every statistic NaN; the clamp keeps 0 * -inf out of t.  Differences come before the product: scores far from zero lose nothing.
+// s and t are float32: at D planes a lane adds D / 16 partial sums to them and moves its maximum D / 16 times at most, 4 roundings of 2^-24
+// each, so that ln s is off by D / 4 + 6 ln D + 40 of them at worst: DT_PLANE_MAX_PLANES keeps that below 1e-3 (64 planes: 5e-6).
 // The G lanes of a group that share a pixel move their maximum together, so that their sums need no rescaling when they join.
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 template <int K>
@@ -247,13 +249,15 @@ struct Stats {
     top = group_max<G>(top);
     if (top != m) rebase(top, c);
     const float m0 = m == -INFINITY ? 0.f : m;
+    float ps = 0.f, pt = 0.f;  // (of these N alone: s and t round once per N planes, not once per plane)
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float y = c * (x[e] - m0);
       const float ex = __builtin_amdgcn_exp2f(y);
-      s += ex;
-      t += ex * fmaxf(y, -1e4f);
+      ps += ex;
+      pt += ex * fmaxf(y, -1e4f);
     }
+    s += ps, t += pt;
     if constexpr (K > 0) {
       static_assert(N % K == 0);
 #pragma unroll
@@ -847,7 +851,7 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
 
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
                              int w, int64_t* plane_bhw, dt_stream_t s) {
-  DT_REQUIRE(b > 0 && d > 0 && d <= DT_PLANE_MAX_PLANES && h > 0 && w > 0, "dt_cv_nearest_planes_f32: bad extents b=%d d=%d h=%d w=%d", b, d, h, w);
+  DT_REQUIRE(b > 0 && d > 0 && d <= DT_PLANE_MAX_NEAREST && h > 0 && w > 0, "dt_cv_nearest_planes_f32: bad extents b=%d d=%d h=%d w=%d", b, d, h, w);
   DT_REQUIRE((int64_t)b * h < INT32_MAX && (int64_t)b * h * w < INT32_MAX, "dt_cv_nearest_planes_f32: more than 2^31 - 1 pixels");
   DT_REQUIRE(depth_bhw && depth_planes && planes_stride4 && plane_bhw, "dt_cv_nearest_planes_f32: null pointer");
   PlaneNear a{depth_bhw, depth_planes, plane_bhw};

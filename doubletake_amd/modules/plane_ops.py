@@ -24,8 +24,8 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_TOP = 8
 #: factors on the scores; the gradient's intermediate values (scale * gradient * log probability) stay finite for gradients up to 1e4
 MIN_SCALE, MAX_SCALE = 1e-30, 1e30
-#: planes per volume (DT_PLANE_MAX_PLANES)
-MAX_PLANES = 1 << 30
+#: planes per volume (DT_PLANE_MAX_PLANES: what float32 sums bear); depth planes nearest_planes searches (DT_PLANE_MAX_NEAREST)
+MAX_PLANES, MAX_NEAREST = 1 << 16, 1 << 30
 
 
 class PlaneLogProbs(NamedTuple):
@@ -161,7 +161,8 @@ _backward_once = torch.autograd.function.once_differentiable(_backward)
 def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=None, depth_planes_bdhw=None) -> PlaneLogProbs:
     """Log probabilities over the depth planes of a volume [b, D, h, w], in one pass over it.
 
-    volume_bdhw: float32, float16 or bfloat16 scores in any layout (NCHW, channels_last, slices); statistics are float32.
+    volume_bdhw: float32, float16 or bfloat16 scores in any layout (NCHW, channels_last, slices), 1..65536 planes; statistics are
+        float32, the log probabilities within 2^-24 (D / 4 + 6 ln D + 40) nats plus 2^-22 of their value.
     plane_bhw: plane indices [b, h, w] (int64 or int32) whose log probability is wanted; one outside 0..D-1 (-1: no depth there)
         scores 0 and takes no part in the gradient.
     top: how many of the most probable planes to return, 0..min(D, 8); equal scores in the order of their planes.
@@ -230,8 +231,8 @@ def nearest_planes(depth_bhw, depth_planes_bdhw):
         raise ValueError(f"depth_bhw must be [b, h, w], got {tuple(depth.shape)}")
     if not depth.is_floating_point():
         raise ValueError(f"depth_bhw is {depth.dtype}; metric depths are floating point")
-    if planes.dim() != 4 or not 1 <= planes.shape[1] <= MAX_PLANES:
-        raise ValueError(f"depth_planes_bdhw must be [b, D, h, w] with 1..{MAX_PLANES} planes, got {tuple(planes.shape)}")
+    if planes.dim() != 4 or not 1 <= planes.shape[1] <= MAX_NEAREST:
+        raise ValueError(f"depth_planes_bdhw must be [b, D, h, w] with 1..{MAX_NEAREST} planes, got {tuple(planes.shape)}")
     if planes.dtype != torch.float32:
         raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
     b, h, w = depth.shape

@@ -217,7 +217,8 @@ int dt_cv_overall_mask_u8(const float* params, const float* depth_planes_bdhw, u
  *   - equal scores: the lowest plane first; alternatives beyond the planes with probability: plane -1, log prob -inf, depth 0. */
 enum { DT_VOL_F32 = 0, DT_VOL_F16 = 1, DT_VOL_BF16 = 2 };
 #define DT_PLANE_MAX_TOP 8
-#define DT_PLANE_MAX_PLANES (1 << 30)
+#define DT_PLANE_MAX_PLANES (1 << 16)  /* of a volume: what float32 sums over the planes bear (ln s within 1e-3) */
+#define DT_PLANE_MAX_NEAREST (1 << 30) /* of dt_cv_nearest_planes_f32, which sums nothing */
 
 typedef struct dt_plane_desc {
   int b, d, h, w;             /* extents of the volume; b * h * w < 2^31 - 1, d <= DT_PLANE_MAX_PLANES */

@@ -224,3 +224,16 @@ def test_backward_refuses_saved_tensors_brought_back_as_others(name, bring, monk
     with pytest.raises(RuntimeError, match="hook on saved tensors"):
         plane_ops._backward(bad, g, g, g, torch.ones(2, 2, 3, 4), None, None)
     assert len(calls) == 1
+
+
+def test_planes_that_float32_sums_do_not_bear_are_refused():
+    """More than 65536 planes: with float32 sums the normaliser would be off by 1e-3 and more, and stop growing at 2^24 of them."""
+    shape = lambda D: torch.zeros(1).expand(1, D, 1, 1)
+    for D in ((1 << 16) + 1, 1 << 20, 1 << 24):
+        with pytest.raises(ValueError, match="planes"):
+            plane_ops.plane_log_probs(shape(D))
+        assert _call(_desc(d=D)) != 0 and _call_grad(_desc(d=D)) != 0
+    with pytest.raises(_abi.DoubletakeHipError, match="CPU"):   # (accepted as far as the device)
+        plane_ops.plane_log_probs(shape(1 << 16))
+    with pytest.raises(_abi.DoubletakeHipError, match="CPU"):   # (a search sums nothing)
+        plane_ops.nearest_planes(torch.ones(1, 1, 1), shape(1 << 24))

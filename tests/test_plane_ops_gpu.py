@@ -591,3 +591,33 @@ def test_more_channels_last_pixels_than_one_grid_takes():
     ref.close(got[at], wg[0, :, 0].T, (err * 1.01 + HALF_STEP[F16] * wg.abs() + TINY[F16])[0, :, 0].T)
     for a, e in ((0, at[80]), (at[159] + 1, at[160]), (at[399] + 1, at[400])):
         assert bool((got[a + 80:e] == 0.5).all())
+
+
+@pytest.mark.parametrize("layout,blocks", [("last", 32), ("first", 64), ("far last", 32), ("far first", 16)])
+@pytest.mark.parametrize("D", [4099, 65536])
+def test_long_sums(D, layout, blocks):
+    """One plane above all others, whose equal terms (0.333 each) a running float32 sum rounds the same way every time.  A lane adds
+    D / ``blocks`` partial sums (lanes per pixel times planes of a partial sum); then joining, the logarithm and the terms' own error as
+    in plane_ref."""
+    x = torch.full((1, D, 1, 3), -1.1)
+    x[:, 7] = 0.0
+    x[0, :, 0, 1] += torch.linspace(-1e-3, 1e-3, D)      # rising a little: the maximum stays plane 7's
+    x[0, :, 0, 2] = torch.linspace(-3, 3, D)             # rising all the way: the maximum moves with every block of planes
+    if layout.startswith("far"):   # (pixels that 32-bit offsets do not reach: one lane per pixel where planes are not innermost)
+        far, step = (1 << 30) + 9, 1 if layout == "far last" else 2
+        vol = torch.zeros(2 * far + 2 * D, dtype=F16, device=DEV).as_strided((1, D, 1, 3), (0, step, 0, far))
+        vol.copy_(x)
+        x = vol.float().cpu()
+    else:
+        vol = x.to(DEV)
+        vol = vol.contiguous(memory_format=torch.channels_last) if layout == "last" else vol.contiguous()
+    plane = torch.full((1, 1, 3), D - 1, device=DEV)
+    r = plane_ops.plane_log_probs(vol, plane, top=2)
+    want = ref.stats(x, plane, 2)
+    rest = 40 + 6 * math.log(D)
+    tol = torch.tensor([D / blocks + rest, D / blocks + rest, 4 * D / blocks + rest]).double().view(1, 1, 3) * ref.U   # (moving: 3 more each)
+    ref.close(r.log_prob_bhw, want["log_prob"], tol + 4 * ref.U * want["log_prob"].abs())
+    ref.close(r.log_sum_bhw, want["log_sum"], tol + 4 * ref.U * (want["log_sum"].abs() + math.log(D)))
+    ref.close(r.top_log_prob_bkhw, want["top_log_prob"], tol + 4 * ref.U * want["top_log_prob"].abs())
+    ref.close(r.entropy_bhw, want["entropy"], tol * (1 + math.log(D)) + 4 * ref.U * (math.log(D) ** 2 + 2))
+    assert torch.equal(r.top_plane_bkhw.cpu(), want["top_plane"])
