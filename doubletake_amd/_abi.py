@@ -32,7 +32,7 @@ class TsdfThresholds(C.Structure):
 class PlaneDesc(C.Structure):
     """struct dt_plane_desc (include/doubletake_hip.h)."""
     _fields_ = [("b", C.c_int), ("d", C.c_int), ("h", C.c_int), ("w", C.c_int), ("dtype", C.c_int), ("top", C.c_int),
-                ("scale", C.c_float), ("pad", C.c_int), ("vol_stride", C.c_int64 * 4), ("mask_stride", C.c_int64 * 4),
+                ("scale", C.c_float), ("outside", C.c_float), ("vol_stride", C.c_int64 * 4), ("mask_stride", C.c_int64 * 4),
                 ("planes_stride", C.c_int64 * 4), ("grad_stride", C.c_int64 * 4)]
 
 

@@ -31,7 +31,7 @@ struct PlaneFwd {
   float *top_depth, *row_max, *row_log;
   int64_t vs[4], ms[4], ps[4];
   int b, d, h, w, top;
-  float scale;
+  float scale, outside;
   Div by_hw, by_w;
   uint32_t first;  // pixel the launch begins at (by_range; 0 with 32-bit offsets)
 };
@@ -284,7 +284,7 @@ __device__ __forceinline__ void write(const PlaneFwd& a, uint32_t p, const Pixel
     store(a.entropy, po, empty ? 0.f : ls - kLn2 * (t * __builtin_amdgcn_rcpf(s)));
     store(a.log_sum, po, m * a.scale + ls);
     if (a.row_max) store(a.row_max, po, m), store(a.row_log, po, ls);
-    if (a.plane) store(a.log_prob, po, given < 0 || given >= a.d ? 0.f : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale));
+    if (a.plane) store(a.log_prob, po, given < 0 || given >= a.d ? a.outside : empty ? -INFINITY : log_prob_of(x_given, m, ls, a.scale));
   }
   if constexpr (K > 0) {
     const Off hw = (Off)a.h * a.w;
@@ -811,7 +811,7 @@ int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint
   DT_REQUIRE(!row_max == !row_log, "dt_cv_plane_log_probs: row_max goes with row_log");
   PlaneFwd a{volume, mask, plane_bhw, depth_planes, log_prob, entropy, log_sum, top_log_prob, top_plane, top_depth, row_max, row_log};
   for (int i = 0; i < 4; ++i) a.vs[i] = d->vol_stride[i], a.ms[i] = d->mask_stride[i], a.ps[i] = d->planes_stride[i];
-  a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale;
+  a.b = d->b, a.d = d->d, a.h = d->h, a.w = d->w, a.top = d->top, a.scale = d->scale, a.outside = d->outside;
   a.by_hw = make_div((uint32_t)d->h * d->w), a.by_w = make_div(d->w);
   by_type(d->dtype, [&](auto v) {
     const bool last = a.vs[1] == 1;

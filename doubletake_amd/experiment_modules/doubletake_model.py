@@ -326,7 +326,8 @@ class _HotPathDepthModel(nn.Module):
         """Add what the cost volume says about its own answer to the outputs of ``forward`` / ``forward_from_features``
         (CostVolumeManager.plane_statistics; no reference counterpart), all float32 at the volume's resolution:
 
-          plane_log_prob_bhw         log probability of the depth plane the predicted depth falls on
+          plane_log_prob_bhw         log probability of the depth plane the predicted depth falls on; -inf where the prediction is no
+                                     depth (not finite or not positive)
           plane_entropy_bhw          entropy of the distribution over planes, nats: 0 = one plane, log D = no plane stands out
           plane_top_log_prob_bkhw,   the ``top`` most probable planes and their depths (top > 0)
           plane_top_depth_bkhw
@@ -350,7 +351,7 @@ class _HotPathDepthModel(nn.Module):
                 break
         else:
             raise ValueError(f"no predicted depth at the cost volume's resolution {h}x{w}: plane statistics need one")
-        r = self.cost_volume.plane_statistics(cost_volume, planes, depth[:, 0], top=top, scale=scale)
+        r = self.cost_volume.plane_statistics(cost_volume, planes, depth[:, 0], top=top, scale=scale, outside=float("-inf"))
         outputs["plane_log_prob_bhw"], outputs["plane_entropy_bhw"] = r.log_prob_bhw, r.entropy_bhw
         if top:
             outputs["plane_top_log_prob_bkhw"], outputs["plane_top_depth_bkhw"] = r.top_log_prob_bkhw, r.top_depth_bkhw

@@ -86,7 +86,8 @@ class FrameTimer:
 def _depth_for_fusion(outputs, size, mask_pred_depth=False, per_view_mask=True, min_plane_log_prob=None):
     """Nearest upsampling of depth_pred_s0 to the ground-truth depth size and the optional masking
     (test_incremental.py:290-294,331-352; test_offline_two_pass.py:97-117).  min_plane_log_prob: depths whose plane the cost
-    volume gives a lower log probability (or NaN) are masked too (``model.enable_plane_statistics``)."""
+    volume gives a lower log probability (or NaN), and predictions that are no depth (not finite or not positive: no plane is theirs),
+    are masked too (``model.enable_plane_statistics``)."""
     depth = outputs["depth_pred_s0_b1hw"]
     if size is not None and tuple(depth.shape[-2:]) != tuple(size):
         depth = F.interpolate(depth, size=tuple(size), mode="nearest")
@@ -103,7 +104,7 @@ def _depth_for_fusion(outputs, size, mask_pred_depth=False, per_view_mask=True, 
         if lp is None:
             raise ValueError("min_plane_log_prob needs plane_log_prob_bhw among the model's outputs: model.enable_plane_statistics()")
         lp = F.interpolate(lp.unsqueeze(1), size=depth.shape[-2:], mode="nearest")
-        depth = torch.where(lp >= min_plane_log_prob, depth, torch.full_like(depth, -1))
+        depth = torch.where((lp >= min_plane_log_prob) & (depth > 0) & (depth < float("inf")), depth, torch.full_like(depth, -1))
     return depth
 
 

@@ -159,14 +159,15 @@ class CostVolumeManager(nn.Module):
     def indices_to_disparity(self, indices, depth_planes_bdhw):
         return torch.gather(depth_planes_bdhw, 1, indices.unsqueeze(1)).squeeze(1)
 
-    def plane_statistics(self, cost_volume, depth_planes_bdhw, depth_bhw=None, top=0, scale=1.0, mask_bdhw=None):
+    def plane_statistics(self, cost_volume, depth_planes_bdhw, depth_bhw=None, top=0, scale=1.0, mask_bdhw=None, outside=0.0):
         """The volume as a distribution over depth planes, next to the one plane ``lowest_cost`` names (no reference counterpart):
         entropy per pixel, the ``top`` most probable planes with their depths and, for a depth map [b, h, w] at the volume's
         resolution (predicted, rendered from a mesh, measured), the log probability of the plane each depth falls on.
-        cost_volume and depth_planes_bdhw: what ``forward`` returns.  Returns plane_ops.PlaneLogProbs."""
+        cost_volume and depth_planes_bdhw: what ``forward`` returns.  outside: the log probability where the depth map has none (not
+        finite or not positive).  Returns plane_ops.PlaneLogProbs."""
         plane = None if depth_bhw is None else plane_ops.nearest_planes(depth_bhw, depth_planes_bdhw)
         return plane_ops.plane_log_probs(cost_volume, plane, top=top, scale=scale, mask_bdhw=mask_bdhw,
-                                         depth_planes_bdhw=depth_planes_bdhw if top else None)
+                                         depth_planes_bdhw=depth_planes_bdhw if top else None, outside=outside)
 
     # -- shared plumbing ---------------------------------------------------------------------
     def _per_batch(self, t, b, dev, slot):

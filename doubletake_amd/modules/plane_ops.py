@@ -30,7 +30,7 @@ MAX_PLANES, MAX_NEAREST = 1 << 16, 1 << 30
 
 class PlaneLogProbs(NamedTuple):
     """What ``plane_log_probs`` returns; entries that were not asked for are None.  Real-valued entries are float32."""
-    log_prob_bhw: Optional[torch.Tensor]        # of the given plane; 0 where it is outside 0..D-1
+    log_prob_bhw: Optional[torch.Tensor]        # of the given plane; ``outside`` (0) where it is not in 0..D-1
     entropy_bhw: torch.Tensor                   # nats
     log_sum_bhw: torch.Tensor                   # log of the sum of exp(scale * score)
     top_log_prob_bkhw: Optional[torch.Tensor]   # descending
@@ -59,10 +59,10 @@ def _broadcast(t, shape, device, name):
     return t.expand(shape)
 
 
-def _desc(vol, top, scale, mask, planes, grad=None):
+def _desc(vol, top, scale, mask, planes, grad=None, outside=0.0):
     d = _abi.PlaneDesc()
     d.b, d.d, d.h, d.w = vol.shape
-    d.dtype, d.top, d.scale = _DTYPES[vol.dtype], top, scale
+    d.dtype, d.top, d.scale, d.outside = _DTYPES[vol.dtype], top, scale, outside
     d.vol_stride[:] = vol.stride()
     if mask is not None:
         d.mask_stride[:] = mask.stride()
@@ -73,7 +73,7 @@ def _desc(vol, top, scale, mask, planes, grad=None):
     return d
 
 
-def _forward(vol, plane, top, scale, mask, planes, for_grad):
+def _forward(vol, plane, top, scale, mask, planes, outside, for_grad):
     """(outputs, row statistics [2, b, h, w] or None, stream)"""
     b, _, h, w = vol.shape
     ent = torch.empty((b, h, w), device=vol.device, dtype=torch.float32)
@@ -94,7 +94,7 @@ def _forward(vol, plane, top, scale, mask, planes, for_grad):
     if b * h * w:
         p = _abi.ptr
         _abi.check(_abi.lib().dt_cv_plane_log_probs(
-            _desc(vol, top, scale, mask, planes), vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
+            _desc(vol, top, scale, mask, planes, None, outside), vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
             stream), "dt_cv_plane_log_probs")
     return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, stream
 
@@ -131,13 +131,13 @@ def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
         _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
             desc, vol.data_ptr(), p(mask), p(plane), ent.data_ptr(), p(tpl), rmax, rmax + 4 * n, p(g_lp), p(g_ent), p(g_lsum), p(g_top),
             grad.data_ptr(), ctx.stream), "dt_cv_plane_log_probs_grad")
-    return grad, None, None, None, None, None
+    return grad, None, None, None, None, None, None
 
 
 class _PlaneLogProbsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, vol, plane, top, scale, mask, planes):
-        out, rows, stream = _forward(vol, plane, top, scale, mask, planes, True)
+    def forward(ctx, vol, plane, top, scale, mask, planes, outside):
+        out, rows, stream = _forward(vol, plane, top, scale, mask, planes, outside, True)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(*[t for t in out[4:] if t is not None])
@@ -158,13 +158,13 @@ class _PlaneLogProbsFn(torch.autograd.Function):
 _backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
-def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=None, depth_planes_bdhw=None) -> PlaneLogProbs:
+def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=None, depth_planes_bdhw=None, outside=0.0) -> PlaneLogProbs:
     """Log probabilities over the depth planes of a volume [b, D, h, w], in one pass over it.
 
     volume_bdhw: float32, float16 or bfloat16 scores in any layout (NCHW, channels_last, slices), 1..65536 planes; statistics are
         float32, the log probabilities within 2^-24 (D / 4 + 6 ln D + 40) nats plus 2^-22 of their value.
     plane_bhw: plane indices [b, h, w] (int64 or int32) whose log probability is wanted; one outside 0..D-1 (-1: no depth there)
-        scores 0 and takes no part in the gradient.
+        scores ``outside`` and takes no part in the gradient.
     top: how many of the most probable planes to return, 0..min(D, 8); equal scores in the order of their planes.
     scale: factor on the scores in front of the softmax (inverse temperature), a positive number, 1e-30..1e30.
     mask_bdhw: bool, broadcastable to the volume; False leaves a plane out, whatever the volume holds there.  A pixel without a
@@ -172,6 +172,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         depth 0) and gradient 0.
     depth_planes_bdhw: float32 depths of the planes, broadcastable to the volume (what the managers return): the alternatives' depths
         are returned too.
+    outside: log probability of a plane index outside 0..D-1: 0 drops such pixels out of a loss, -inf says that no plane is certain there.
 
     Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice): the gradient has the volume's
     type and layout.  A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on
@@ -189,7 +190,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
     top = int(top)
     if not 0 <= top <= min(D, MAX_TOP):
         raise ValueError(f"top={top} not in 0..{min(D, MAX_TOP)}")
-    scale = float(scale)
+    scale, outside = float(scale), float(outside)
     check_scale(scale)
     plane = plane_bhw
     if plane is not None:
@@ -217,8 +218,8 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         planes = _broadcast(planes, vol.shape, vol.device, "depth_planes_bdhw")
     _require_gpu(vol, "volume_bdhw")
     if vol.requires_grad and torch.is_grad_enabled():
-        return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes))
-    return _forward(vol, plane, top, scale, mask, planes, False)[0]
+        return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes, outside))
+    return _forward(vol, plane, top, scale, mask, planes, outside, False)[0]
 
 
 @torch.no_grad()

@@ -213,7 +213,7 @@ int dt_cv_overall_mask_u8(const float* params, const float* depth_planes_bdhw, u
  *   - masked planes may hold anything (NaN, infinities); a score of -inf is a plane without probability;
  *   - a pixel without any probability: log_sum = log_prob = -inf, entropy = 0, no alternatives, gradient 0;
  *   - a visible NaN or +inf makes the pixel's real-valued outputs NaN (the order of the alternatives stays defined: NaN first);
- *   - a given plane outside 0..d-1 scores nothing: log_prob = 0, no gradient;
+ *   - a given plane outside 0..d-1 scores nothing: log_prob = dt_plane_desc.outside, no gradient;
  *   - equal scores: the lowest plane first; alternatives beyond the planes with probability: plane -1, log prob -inf, depth 0. */
 enum { DT_VOL_F32 = 0, DT_VOL_F16 = 1, DT_VOL_BF16 = 2 };
 #define DT_PLANE_MAX_TOP 8
@@ -225,7 +225,7 @@ typedef struct dt_plane_desc {
   int dtype;                  /* DT_VOL_*: type of the volume and of its gradient */
   int top;                    /* alternatives per pixel, 0..min(d, DT_PLANE_MAX_TOP) */
   float scale;                /* inverse temperature, 1e-30..1e30 */
-  int pad;
+  float outside;              /* log_prob where the given plane is outside 0..d-1: 0 for losses, -inf where certainty is asked for */
   int64_t vol_stride[4];      /* elements between neighbours along b, d, y, x: any layout, none negative */
   int64_t mask_stride[4];     /* bytes, likewise; 0 along a broadcast axis */
   int64_t planes_stride[4];   /* elements of the depth planes, likewise */

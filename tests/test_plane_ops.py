@@ -237,3 +237,16 @@ def test_planes_that_float32_sums_do_not_bear_are_refused():
         plane_ops.plane_log_probs(shape(1 << 16))
     with pytest.raises(_abi.DoubletakeHipError, match="CPU"):   # (a search sums nothing)
         plane_ops.nearest_planes(torch.ones(1, 1, 1), shape(1 << 24))
+
+
+@pytest.mark.parametrize("size", [None, (4, 6)])
+def test_loops_mask_predictions_that_are_no_depth(size):
+    """A log probability of 0 (what an operator reports for a pixel without a plane) does not make a NaN or infinite depth certain."""
+    from doubletake_amd import loops
+
+    depth = torch.tensor([[1.0, math.nan, math.inf], [-math.inf, 0.0, -2.0]]).view(1, 1, 2, 3)
+    got = loops._depth_for_fusion({"depth_pred_s0_b1hw": depth, "plane_log_prob_bhw": torch.zeros(1, 2, 3)}, size, min_plane_log_prob=-1.0)
+    want = torch.tensor([[1.0, -1, -1], [-1, -1, -1]]).view(1, 1, 2, 3)
+    if size:
+        want = want.repeat_interleave(2, 2).repeat_interleave(2, 3)
+    assert torch.equal(got, want)

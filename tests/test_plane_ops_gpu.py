@@ -621,3 +621,21 @@ def test_long_sums(D, layout, blocks):
     ref.close(r.top_log_prob_bkhw, want["top_log_prob"], tol + 4 * ref.U * want["top_log_prob"].abs())
     ref.close(r.entropy_bhw, want["entropy"], tol * (1 + math.log(D)) + 4 * ref.U * (math.log(D) ** 2 + 2))
     assert torch.equal(r.top_plane_bkhw.cpu(), want["top_plane"])
+
+
+@pytest.mark.parametrize("layout", ["last", "first"])
+@pytest.mark.parametrize("shape", [(2, 20, 5, 7), (1, 40, 200, 210)], ids=str)
+def test_log_probability_of_planes_outside(shape, layout):
+    vol, m, plane, _ = make(shape, layout=layout, mask="plane", seed=48)
+    base = plane_ops.plane_log_probs(vol, plane, top=2, mask_bdhw=m)
+    out = (plane < 0) | (plane >= shape[1])
+    assert bool(out.any()) and bool((base.log_prob_bhw[out] == 0).all())
+    for value in (-math.inf, 2.5, math.nan):
+        leaf = vol.detach().requires_grad_(True)
+        for v in (vol, leaf):
+            r = plane_ops.plane_log_probs(v, plane, top=2, mask_bdhw=m, outside=value)
+            assert bool((r.log_prob_bhw[out] == value).all()) if value == value else bool(r.log_prob_bhw[out].isnan().all())
+            assert torch.equal(r.log_prob_bhw[~out], base.log_prob_bhw[~out])
+            assert all(torch.equal(a, b) for a, b in zip(r[1:5], base[1:5]))
+        grad, = torch.autograd.grad(r.log_prob_bhw, leaf, torch.ones_like(r.log_prob_bhw))
+        assert bool((grad.permute(0, 2, 3, 1)[out] == 0).all()) and bool(torch.isfinite(grad).all())

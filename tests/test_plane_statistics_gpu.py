@@ -194,3 +194,24 @@ def test_losses_on_the_volume_reach_the_features():
     # D products of gradient (error: a few float32 steps of values below 1.5 / 114 pixels ...) and feature (below 5), summed over D planes
     tol = D * 5 * (1.5 / 100) * 64 * 2.0 ** -24 + D * 5 * (1.5 / 100) * ref.bound_b(D)
     assert float((a.grad.double() - e.grad).abs().max()) < tol
+
+
+def test_predictions_that_are_no_depth_are_not_certain():
+    """NaN, infinite, zero and negative predictions fall on no plane: log probability -inf in the model's outputs, masked by the loops."""
+    from doubletake_amd import loops
+
+    model, frame, run, volume = _model(b=2)
+    model.enable_plane_statistics(top=0)
+    fr = frame(6)
+    out = run(fr)
+    vol, _, planes, _ = volume(fr)
+    depth = out["depth_pred_s1_b1hw"].clone()
+    bad = torch.zeros_like(depth, dtype=torch.bool)
+    for k, v in enumerate((float("nan"), float("inf"), -float("inf"), 0.0, -1.0)):
+        depth[:, :, k, 3:9] = v
+        bad[:, :, k, 3:9] = True
+    got = model._add_plane_statistics({"depth_pred_s1_b1hw": depth}, vol, planes)["plane_log_prob_bhw"]
+    assert bool((got[bad[:, 0]] == -float("inf")).all())
+    assert torch.equal(got[~bad[:, 0]], out["plane_log_prob_bhw"][~bad[:, 0]])
+    full = loops._depth_for_fusion(dict(out, plane_log_prob_bhw=got), (24, 32), min_plane_log_prob=-1e30)
+    assert bool((full[bad] == -1).all()) and bool((full[~bad] > 0).all())
