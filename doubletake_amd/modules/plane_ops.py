@@ -16,6 +16,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from .. import _abi
 
@@ -46,6 +47,12 @@ def check_scale(scale):
 def _require_gpu(t, name):
     if not t.is_cuda:
         raise _abi.DoubletakeHipError(f"{name} is on {t.device}; doubletake_amd plane statistics only run on a ROCm GPU (no CPU fallback)")
+
+
+def _refuse_tangent(t, name):
+    # (a comparison outside forward mode: unpack_dual costs 3 us)
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} carries a forward-mode tangent: plane_ops has reverse-mode gradients only")
 
 
 def _broadcast(t, shape, device, name):
@@ -178,7 +185,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         are returned too.
     outside: log probability of a plane index outside 0..D-1: 0 drops such pixels out of a loss, -inf says that no plane is certain there.
 
-    Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice): the gradient has the volume's
+    Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice, not in forward mode): the gradient has the volume's
     type and layout.  A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on
     the current stream (planes innermost: one per 2^29 pixels) and can be captured into a graph; capture a backward pass only together with its forward pass."""
     vol = volume_bdhw
@@ -220,6 +227,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         if planes.dtype != torch.float32:
             raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
         planes = _broadcast(planes, vol.shape, vol.device, "depth_planes_bdhw")
+    _refuse_tangent(vol, "volume_bdhw")
     _require_gpu(vol, "volume_bdhw")
     if vol.requires_grad and torch.is_grad_enabled():
         return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes, outside))

@@ -250,3 +250,21 @@ def test_loops_mask_predictions_that_are_no_depth(size):
     if size:
         want = want.repeat_interleave(2, 2).repeat_interleave(2, 3)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_forward_mode_tangents_are_refused(needs_grad):
+    """They would be dropped without a word; the volume without one is taken as ever (as far as the device, here)."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        v = _vol()
+        dual = forward_ad.make_dual(v.requires_grad_(needs_grad), torch.ones_like(v))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            plane_ops.plane_log_probs(dual)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+            plane_ops.plane_log_probs(dual)
+        with pytest.raises(_abi.DoubletakeHipError):
+            plane_ops.plane_log_probs(_vol())
+    with pytest.raises(NotImplementedError, match="tangent"):
+        torch.func.jvp(lambda x: plane_ops.plane_log_probs(x).entropy_bhw, (_vol(),), (_vol(),))
