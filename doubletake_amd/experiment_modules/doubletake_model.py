@@ -97,6 +97,8 @@ class _HotPathDepthModel(nn.Module):
                    "matching_encoder_type", "feature_volume_type")
     _VOLUME_TYPES = ()
     _DEFAULT_VOLUME_TYPE = None
+    #: (top, scale) while enable_plane_statistics is on
+    _plane_statistics = None
 
     def __init__(self, image_height=384, image_width=512, image_encoder_name="resnet18d", depth_decoder_name="skip",
                  matching_num_depth_bins=64, matching_scale=1, matching_feature_dims=16, model_num_views=8,
@@ -333,7 +335,7 @@ class _HotPathDepthModel(nn.Module):
           plane_top_depth_bkhw
 
         ``scale``: factor on the volume's scores in front of the softmax.  Two more launches per call; works under captured graphs and
-        launch programs.  ``loops`` can mask depths by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
+        launch programs, and for a driver of the two stages (volume_stage then returns the depth planes too).  ``loops`` can mask depths by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
         top, scale = int(top), float(scale)
         if on and not 0 <= top <= min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins):
             raise ValueError(f"top={top} not in 0..{min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins)}")
@@ -359,7 +361,7 @@ class _HotPathDepthModel(nn.Module):
 
     def _launch_config(self):
         cv = self.cost_volume
-        return ops.launch_config() + (getattr(self, "_plane_statistics", None), getattr(cv, "precision", None), getattr(cv, "use_span_plan", None),
+        return ops.launch_config() + (self._plane_statistics, getattr(cv, "precision", None), getattr(cv, "use_span_plan", None),
                                       getattr(cv, "channels_last_output", None))
 
     def enable_launch_programs(self, on=True):
@@ -484,11 +486,10 @@ class _HotPathDepthModel(nn.Module):
                   return_mask=return_mask)
         if isinstance(self.cost_volume, FeatureMeshHintVolumeManager):  # the other managers take no hints
             kw["cv_depth_hint_dict"] = cv_depth_hint_dict
-        statistics = getattr(self, "_plane_statistics", None) is not None
-        if statistics:  # (volume_stage keeps the planes to itself)
-            cost_volume, lowest_cost, planes, overall_mask = self.cost_volume(**kw)
-        else:
-            cost_volume, lowest_cost, overall_mask = self.volume_stage(kw)
+        stage = self.volume_stage(kw)
+        if self._plane_statistics is not None and len(stage) < 4:
+            raise ValueError("plane statistics need the depth planes: while they are on, volume_stage returns (cost_volume, lowest_cost, "
+                             "overall_mask, depth_planes_bdhw)")
         # graph mode: the replay is split here so that the hook below runs between the halves -- only when a hook is
         # waiting at capture time (every cut is one more hipGraphLaunch per replay)
         if "after_volume" in self.__dict__ or _graphs.recording():
@@ -499,9 +500,9 @@ class _HotPathDepthModel(nn.Module):
             # and all of its LDS) and beside the conv stack that follows (latency-bound, most of the chip idle):
             # loops.matching_lookahead encodes the next frame's keyframe here
             hook()
-        outputs = self.network_stage(cur_feats, cost_volume, lowest_cost, overall_mask)
-        if statistics:
-            self._add_plane_statistics(outputs, cost_volume, planes)
+        outputs = self.network_stage(cur_feats, *stage[:3])
+        if self._plane_statistics is not None:
+            self._add_plane_statistics(outputs, stage[0], stage[3])
         return outputs
 
     # The two halves of the forward pass, callable on their own so that a driver with several keyframes in flight can order
@@ -509,13 +510,17 @@ class _HotPathDepthModel(nn.Module):
     # stack that follows is a chain of latency-bound launches that several frames can share.
     @torch.no_grad()
     def volume_stage(self, volume_kwargs):
-        """cost volume + lowest cost + mask of one keyframe batch (kwargs of self.cost_volume)."""
-        cost_volume, lowest_cost, _, overall_mask = self.cost_volume(**volume_kwargs)
+        """cost volume + lowest cost + mask of one keyframe batch (kwargs of self.cost_volume); with plane statistics on the volume's
+        depth planes come fourth.  The one way to the volume, of forward_from_features too: a replacement returns the same."""
+        cost_volume, lowest_cost, planes, overall_mask = self.cost_volume(**volume_kwargs)
+        if self._plane_statistics is not None:
+            return cost_volume, lowest_cost, overall_mask, planes
         return cost_volume, lowest_cost, overall_mask
 
     @torch.no_grad()
-    def network_stage(self, cur_feats, cost_volume, lowest_cost, overall_mask):
-        """CVEncoder + depth decoder + exp on the volume of volume_stage -> the reference's output dict."""
+    def network_stage(self, cur_feats, cost_volume, lowest_cost, overall_mask, depth_planes_bdhw=None):
+        """CVEncoder + depth decoder + exp on the volume of volume_stage -> the reference's output dict, with the plane statistics
+        where they are on and volume_stage's planes are passed along: ``network_stage(cur_feats, *volume_stage(kwargs))``."""
         cv_feats = self.cost_volume_net(cost_volume, cur_feats[self.matching_scale:])
         feats = list(cur_feats[: self.matching_scale]) + cv_feats
         depth_outputs = self.depth_decoder(feats, with_depth=True)  # heads write exp(log depth) themselves
@@ -528,6 +533,8 @@ class _HotPathDepthModel(nn.Module):
                 depth_outputs[k.replace("log_", "")] = ops.exp(log_depth)
         depth_outputs["lowest_cost_bhw"] = lowest_cost
         depth_outputs["overall_mask_bhw"] = overall_mask
+        if depth_planes_bdhw is not None and self._plane_statistics is not None:
+            self._add_plane_statistics(depth_outputs, cost_volume, depth_planes_bdhw)
         return depth_outputs
 
     @staticmethod

@@ -215,3 +215,19 @@ def test_predictions_that_are_no_depth_are_not_certain():
     assert torch.equal(got[~bad[:, 0]], out["plane_log_prob_bhw"][~bad[:, 0]])
     full = loops._depth_for_fusion(dict(out, plane_log_prob_bhw=got), (24, 32), min_plane_log_prob=-1e30)
     assert bool((full[bad] == -1).all()) and bool((full[~bad] > 0).all())
+
+
+def test_the_two_stages_driven_apart_equal_forward():
+    model, frame, run, _ = _model(b=2)
+    model.enable_plane_statistics(top=2)
+    fr = frame(8)
+    want = run(fr)
+    seen = []
+    kept = model.volume_stage
+    model.volume_stage = lambda kw: seen.append(kw) or kept(kw)
+    out = run(fr)
+    assert len(seen) == 1 and all(torch.equal(out[k], want[k]) for k in KEYS)
+    out = model.network_stage(fr[1], *kept(seen[0]))
+    assert set(out) == set(want)
+    for k, v in want.items():
+        assert torch.equal(out[k], v), k
