@@ -675,7 +675,8 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
 }
 
 // ---- planes of depths ------------------------------------------------------------------------------------------------------------
-// 64-bit differences of 32-bit depths are exact wherever two of them are close, so a tie is a tie; 16 planes' loads are in flight together.
+// 64-bit differences of 32-bit depths are exact within a factor of 2^29 (24 + 29 = 53 bits), so a tie is a tie there; beyond, rounding keeps
+// the order of the differences but may make equal ones of them.  16 planes' loads are in flight together.
 // Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 4.6 us, 5.1 with four waves).
 // Bound: memory where planes vary over the image (8 x 96 x 240 x 320: 46 us, 5.2 TB/s, a part from the last-level cache), else latency.
 __global__ void __launch_bounds__(64) nearest_planes_kernel(PlaneNear a) {

@@ -236,8 +236,9 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
 
 @torch.no_grad()
 def nearest_planes(depth_bhw, depth_planes_bdhw):
-    """int64 [b, h, w]: index of the depth plane nearest to each depth (absolute difference, the lowest index of equally near ones), the depths taken in float32;
-    -1 where the depth is not finite or not positive (holes of a sensor's map, a renderer's background).  depth_planes_bdhw is
+    """int64 [b, h, w]: index of the depth plane nearest to each depth (absolute difference, the lowest index of equally near ones), the depths taken in
+    float32 and the differences in float64: exact within a factor of 2^29, beyond it planes whose distances round to the same number are
+    equally near (all planes of a few metres to a depth of 1e20: plane 0); -1 where the depth is not finite or not positive (holes of a sensor's map, a renderer's background).  depth_planes_bdhw is
     float32 and broadcastable to [b, D, h, w] (what the cost-volume managers return)."""
     depth, planes = depth_bhw, depth_planes_bdhw
     if depth.dim() != 3:

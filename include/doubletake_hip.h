@@ -248,8 +248,9 @@ int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const
                                const float* entropy, const int64_t* top_plane, const float* row_max, const float* row_log,
                                const float* g_log_prob, const float* g_entropy, const float* g_log_sum, const float* g_top_log_prob,
                                void* grad_volume, dt_stream_t s);
-/* The plane a metric depth falls on: argmin_d |depth - planes_d| per pixel (differences in 64 bits: exact), the lowest plane of
- * equal ones; -1 where the depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x;
+/* The plane a metric depth falls on: argmin_d |depth - planes_d| per pixel, the lowest plane of equal ones.  Differences are taken in
+ * 64 bits: exact for planes within a factor of 2^29 of the depth, rounded beyond, so that planes whose distances differ by less than
+ * a step of 64 bits count as equally near (a depth of 1e20 is equally far from all planes of a few metres: plane 0).  -1 where the depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x;
  * 0 along a broadcast axis, none negative); a plane that is no finite number is never the nearest. */
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
                              int w, int64_t* plane_bhw, dt_stream_t s);

@@ -1,5 +1,6 @@
 """plane_ops on the GPU against the 64-bit form in plane_ref (its error bounds are derived there)."""
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -639,3 +640,24 @@ def test_log_probability_of_planes_outside(shape, layout):
             assert all(torch.equal(a, b) for a, b in zip(r[1:5], base[1:5]))
         grad, = torch.autograd.grad(r.log_prob_bhw, leaf, torch.ones_like(r.log_prob_bhw))
         assert bool((grad.permute(0, 2, 3, 1)[out] == 0).all()) and bool(torch.isfinite(grad).all())
+
+
+@pytest.mark.parametrize("order", ["ascending", "descending", "mixed"])
+def test_nearest_planes_of_far_depths(order):
+    """By fractions: the nearest plane exactly where depth and planes are within a factor of 2^29, never farther than the nearest by more
+    than a step of 64 bits beyond it, and the lowest of the planes whose distances round to the same number."""
+    planes = (0.25 * 20.0 ** torch.linspace(0, 1, 33)).float()
+    planes = {"ascending": planes, "descending": planes.flip(0), "mixed": planes[torch.arange(33) * 7 % 33]}[order]
+    depths = [0.1, 1.37, 5.0, 7.0, 1e3, 1e6, 1.3e8, 1e9, 1e12, 1e16, 1e20, 1e30, 3e38, 1e-12, 1e-30, 1e-45]
+    dep = torch.tensor(depths, dtype=F32).view(1, 1, -1)
+    got = plane_ops.nearest_planes(dep.to(DEV), planes.view(1, -1, 1, 1).to(DEV)).view(-1).tolist()
+    exact = [Fraction(float(p)) for p in planes]
+    for z, at in zip((Fraction(float(v)) for v in dep.view(-1)), got):
+        far = [abs(p - z) for p in exact]
+        if max(exact) < z * 2 ** 29 and z < min(exact) * 2 ** 29:
+            assert at == far.index(min(far)), float(z)
+        assert far[at] <= min(far) * (1 + Fraction(1, 2 ** 52)), float(z)
+        rounded = [float(f) for f in far]   # (to nearest, like the kernel's one subtraction)
+        assert at == rounded.index(min(rounded)), float(z)
+    if order == "ascending":
+        assert got[:7] == [0, got[1], 32, 32, 32, 32, 32] and got[-6:] == [0] * 6
