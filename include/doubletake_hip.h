@@ -233,25 +233,28 @@ typedef struct dt_plane_desc {
 } dt_plane_desc;
 
 /* Statistics of every pixel in one pass over the volume.  mask (1 byte per plane, 0 = not visible), plane_bhw and depth_planes may
- * be NULL; depth_planes is read for the alternatives' depths only.  Outputs are dense: log_prob (with plane_bhw only), entropy and
- * log_sum [b,h,w]; top_log_prob, top_plane and (with depth_planes) top_depth [b,top,h,w]; row_max and row_log [b,h,w] (both or
- * neither) are m and ln s, what ..._grad needs.  Any output but entropy and log_sum may be NULL where it is not wanted. */
+ * be NULL; depth_planes is read for the alternatives' depths only.  Outputs are dense; entropy and log_sum [b,h,w] are always
+ * written.  log_prob [b,h,w] goes with plane_bhw: both or neither.  With top > 0 top_log_prob and top_plane [b,top,h,w] are both
+ * required; top_depth [b,top,h,w] may be NULL and needs depth_planes.  row_max and row_log [b,h,w], both or neither, are m and
+ * ln s, what ..._grad needs. */
 int dt_cv_plane_log_probs(const dt_plane_desc* d, const void* volume, const uint8_t* mask, const int64_t* plane_bhw,
                           const float* depth_planes, float* log_prob, float* entropy, float* log_sum, float* top_log_prob,
                           int64_t* top_plane, float* top_depth, float* row_max, float* row_log, dt_stream_t s);
 /* Gradient of the volume for gradients of the outputs above (each NULL where there is none; dense, shaped like its output):
  *   dx_d = scale [ sum of the gradients that meet plane d (given plane, alternatives)
  *                  + p_d (g_log_sum - g_log_prob - sum g_top) - g_entropy p_d (lp_d + entropy) ]
- * mask, plane_bhw, entropy, top_plane, row_max and row_log are those of the forward call.  Every element of the gradient is
- * written (0 for masked planes). */
+ * mask, plane_bhw, entropy, top_plane, row_max and row_log are those of the forward call; g_log_prob needs plane_bhw, g_top_log_prob
+ * needs top_plane, without them either may be NULL.  Every element of the gradient is written (0 for masked planes and scores of
+ * -inf). */
 int dt_cv_plane_log_probs_grad(const dt_plane_desc* d, const void* volume, const uint8_t* mask, const int64_t* plane_bhw,
                                const float* entropy, const int64_t* top_plane, const float* row_max, const float* row_log,
                                const float* g_log_prob, const float* g_entropy, const float* g_log_sum, const float* g_top_log_prob,
                                void* grad_volume, dt_stream_t s);
 /* The plane a metric depth falls on: argmin_d |depth - planes_d| per pixel, the lowest plane of equal ones.  Differences are taken in
  * 64 bits: exact for planes within a factor of 2^29 of the depth, rounded beyond, so that planes whose distances differ by less than
- * a step of 64 bits count as equally near (a depth of 1e20 is equally far from all planes of a few metres: plane 0).  -1 where the depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x;
- * 0 along a broadcast axis, none negative); a plane that is no finite number is never the nearest. */
+ * a step of 64 bits count as equally near (a depth of 1e20 is equally far from all planes of a few metres: plane 0).  -1 where the
+ * depth is not finite or not positive.  depth dense [b,h,w]; planes read through planes_stride4 (b, d, y, x; 0 along a broadcast
+ * axis, none negative), at most DT_PLANE_MAX_NEAREST; a plane that is no finite number is never the nearest. */
 int dt_cv_nearest_planes_f32(const float* depth_bhw, const float* depth_planes, const int64_t* planes_stride4, int b, int d, int h,
                              int w, int64_t* plane_bhw, dt_stream_t s);
 

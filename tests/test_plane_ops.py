@@ -331,3 +331,16 @@ def test_the_two_stages_driven_apart_yield_statistics(monkeypatch):
     assert "plane_log_prob_bhw" not in m.network_stage([None] * 5, *stage[:3])
     m.enable_plane_statistics(False)
     assert "plane_log_prob_bhw" not in m.network_stage([None] * 5, *stage)
+
+
+def test_header_states_which_outputs_go_together():
+    """The refusals of test_abi_refuses_pointers, as a C caller reads them."""
+    import os
+    import re
+
+    text = open(os.path.join(os.path.dirname(__file__), "..", "include", "doubletake_hip.h")).read()
+    words = re.sub(r"[\s*]+", " ", text[text.index("Statistics of every pixel"):text.index("int dt_cv_plane_log_probs(")])
+    assert "may be NULL where it is not wanted" not in words
+    for says in ("log_prob [b,h,w] goes with plane_bhw: both or neither", "top_log_prob and top_plane [b,top,h,w] are both required",
+                 "top_depth [b,top,h,w] may be NULL and needs depth_planes", "row_max and row_log [b,h,w], both or neither"):
+        assert says in words, says
