@@ -146,7 +146,7 @@ SIGNATURES = {
 
 
 # = DT_ABI_VERSION of include/doubletake_hip.h (tests/test_abi.py compares the two)
-ABI_VERSION = 105
+ABI_VERSION = 106
 
 
 def lib():

@@ -28,13 +28,13 @@ extern "C" {
 typedef void* dt_stream_t; /* hipStream_t */
 
 /* ---- library ------------------------------------------------------------------------ */
-/* ABI version: bumped whenever the signature of ANY entry point below changes (not for new entry points alone).
+/* ABI version: bumped whenever the signature of ANY entry point or a struct below changes (not for new entry points alone).
  * Bindings compare it with the version they were written against before the first call: an older .so called with
  * shifted arguments would corrupt device memory instead of failing.  History: 101 round 2; 102 round 3 (depth_planes /
  * channels arguments of dt_cv_lowest_cost_f32, dt_cv_overall_mask_u8, dt_cv_mlp_hint_simple_f32); 103 round 4;
  * 104 plan_scratch_bytes argument of dt_cv_mlp_hint_planned_f32; 105 the plan is written by dt_cv_mlp_plan_f32, the planned
- * call only consumes it. */
-#define DT_ABI_VERSION 105
+ * call only consumes it; 106 dt_plane_desc.outside in the place of padding, which a caller could leave unset. */
+#define DT_ABI_VERSION 106
 int dt_version(void);
 const char* dt_last_error(void);
 /* number of HIP devices visible; <0 on runtime error.  No other call needs it. */
