@@ -334,6 +334,10 @@ class _HotPathDepthModel(nn.Module):
           plane_top_log_prob_bkhw,   the ``top`` most probable planes and their depths (top > 0)
           plane_top_depth_bkhw
 
+        Every pixel counts: the overall mask is not applied (nor does ``return_mask`` change anything), so a pixel that no source view sees
+        has the statistics of whatever the volume scores there.  Statistics of seen pixels alone:
+        ``CostVolumeManager.plane_statistics(..., mask_bdhw=)``; in the loops ``mask_pred_depth`` drops the others.
+
         ``scale``: factor on the volume's scores in front of the softmax.  Two more launches per call; works under captured graphs and
         launch programs, and for a driver of the two stages (volume_stage then returns the depth planes too).  ``loops`` can mask depths by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
         top, scale = int(top), float(scale)

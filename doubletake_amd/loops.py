@@ -236,7 +236,8 @@ def run_incremental_scan(model_fn, fuser, batches, render_hw, fuse_size=None, fu
     (test_incremental.py:205,256-258,274-288).  lookahead: callable(next_cur_data, next_src_data) run before the model of
     the current frame -- work of frame t+1 that does not depend on frame t's result (``matching_lookahead``: its matching
     features) and can fill the chip beside frame t's latency-bound kernels.  min_plane_log_prob: depths whose plane the cost
-    volume gives a lower log probability are not fused (needs ``model.enable_plane_statistics()``).  Returns the number of
+    volume gives a lower log probability are not fused (needs ``model.enable_plane_statistics()``; it knows nothing of pixels that no
+    source view sees, which ``mask_pred_depth`` drops).  Returns the number of
     frames fused."""
     scan = IncrementalScan(model_fn, fuser, batches, render_hw, fuse_size=fuse_size, fused_hint=fused_hint,
                            mask_pred_depth=mask_pred_depth, on_frame=on_frame, timer=timer, lookahead=lookahead,
