@@ -284,3 +284,13 @@ def test_hot_path_kernels_do_not_spill():
     assert all(n > 0 for n in seen.values()), {k: v for k, v in seen.items() if v == 0}
     assert not bad, bad
     assert not any("conv_wino_kernelILi4E" in n for n in notes)  # (the experimental 1024-thread instantiation is gone)
+
+
+def test_build_entry_compiles_even_where_a_library_is_built(monkeypatch):
+    import __graft_entry__
+    from doubletake_amd import _build
+
+    asked = []
+    monkeypatch.setattr(_build, "build", lambda force=False, verbose=True: asked.append(force) or _build.LIB)
+    __graft_entry__.build()
+    assert asked == [True]
