@@ -24,7 +24,7 @@ HASHFILE = os.path.join(LIBDIR, "build_hash.txt")
 # cost extra issue cycles beside MFMAs on gfx950 (MI355X_MICROARCH.md, "price of one filler beside MFMAs");
 # measured on the volume kernel: 0.807 -> 0.795 ms
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 at all -- with SLP off they still come out of vector-typed code (1280 of them in the
-# dot-product volume), and some of their operand forms have given wrong results on this hardware now and then
+# dot-product volume).  A precaution: no kernel here relies on their operand forms
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-fno-slp-vectorize",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extras.  tsdf.hip restates the reference's half pipeline op by op: fusing a multiply

@@ -10,7 +10,8 @@
 
 namespace dt {
 
-// unsigned division by a launch constant (multiply, add, shift) for numerators below 2^31
+// unsigned division by a launch constant (multiply, add, shift) for numerators below 2^31: the round-up method of Granlund and Montgomery,
+// Division by Invariant Integers using Multiplication, 1994
 struct Div {
   uint32_t mul, shift;
 };
@@ -108,8 +109,9 @@ __device__ __forceinline__ uint32_t quad_pixel(const A& a) {
 
 // A launch-uniform 64-bit base plus an offset in bytes per lane.  The empty statement keeps the base in scalar registers: left to itself
 // the compiler adds the two first, a 64-bit vector addition and two registers per access, and hoists the sums out of the loop over
-// planes.  Planes innermost, D = 64, 4 alternatives, 8 x 120 x 160 pixels: 80 -> 54 registers, 13.6 -> 12.9 us.  (Not where a lane steps
-// over planes, the hoisted addresses win there: 128 planes of float16, 8 x 240 x 320 pixels 36.4 us, kept in scalar registers 39.9.)
+// planes.  Planes innermost, D = 64, 4 alternatives, 8 x 120 x 160 pixels: 60 -> 56 registers and 13.6 -> 13.4 us, with a mask per plane
+// 83 -> 66 and 15.9 -> 15.7.  (Not where a lane steps over planes, the hoisted addresses win there: 128 planes of float16, 8 x 240 x 320
+// pixels 36.3 us, kept in scalar registers 39.0.)
 #define DT_GLOBAL __attribute__((address_space(1)))
 template <typename T, typename Off>
 __device__ __forceinline__ T load(const void* base, Off off) {
@@ -378,7 +380,7 @@ struct Spread {
 };
 // What the readers below know about the mask at compile time: none that varies over the planes, one byte per load, or the planes' bytes
 // next to each other like the scores (a comparison of a channels_last volume): then as many bytes per load as scores, taken apart when
-// they are used.  One kernel for all three held the addresses and branches of each: 4 alternatives, 8 x 64 x 120 x 160: 14.8 us, 13.6 apart.
+// they are used.  (One kernel for all three would hold the addresses and branches of each.)
 enum MaskKind { kNoMask, kMaskBytes, kMaskVectors };
 template <MaskKind M, typename T, int G, int N, typename Off, typename A>
 __device__ __forceinline__ void load_last(Raw<T, N>& raw, const A& a, int d0, int lane, Off vo, Off mo) {
@@ -461,9 +463,10 @@ __device__ __forceinline__ void add_planes(Stats<K>& st, const float (&x)[kN], f
 // Volume with neighbouring pixels next to each other (NCHW; any strides work): one lane per pixel.
 // S = 4: the four waves of a workgroup share 64 pixels, a quarter of the planes each; the partial results change places through LDS so
 // that four neighbouring lanes hold the four parts of a pixel, and all waves join and write 16 pixels each.
-// Bound: memory in float32 (16 x 64 x 120 x 160 pixels, 4 alternatives: 21.3 us, 4.7 TB/s of what has to move; a large copy on this card
-// reaches 4.8) and in float16 without alternatives (8 x 128 x 240 x 320: 36.6 us, 4.6 TB/s); vector instructions in float16 with
-// alternatives (16 x 64 x 120 x 160, 4 of them: 19.1 us, 3.1 TB/s); latency below about 50000 pixels (one keyframe 3.5 to 4.7 us).
+// Bound: memory in float32 (16 x 64 x 120 x 160 pixels, 4 alternatives: 21.2 us, 4.7 TB/s of what has to move; a large copy on this card
+// reaches 4.8) and in float16 without alternatives (8 x 128 x 240 x 320: 36.3 us, 4.7 TB/s).  In float16 with alternatives (16 x 64 x 120
+// x 160, 4 of them: 20.0 us, 3.0 TB/s) memory (12.5 us) and vector instructions (1538 a wave, 12.5 us) take turns: a lane has nothing in
+// flight during its arithmetic, and 4.7 waves per SIMD cover a part.  Latency below about 50000 pixels (one keyframe 4.2 to 5.3 us).
 template <typename T, int K, int S, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -517,10 +520,10 @@ __global__ void __launch_bounds__(256) plane_stats_first_kernel(PlaneFwd a) {
 }
 
 // Volume with the planes of a pixel next to each other (channels_last): four lanes per pixel, 8 planes per lane at a time.  Two loads of
-// a lane cover the halves of a 128-byte line, so four lanes fetch whole lines; 16 lanes per pixel paid more for joining and writing
-// (8 x 64 x 120 x 160, 4 alternatives, an early version: 55 us against 19), two lanes and 16 planes at a time were within 10 % either way.
-// Bound: memory from about 64 float32 planes on (16 x 64 x 120 x 160, 4 alternatives: 20.7 us, 4.8 TB/s), the vector instructions of
-// joining and writing a pixel below (8 x 32 x 120 x 160: 9.3 us, 3.2 TB/s) and in 16 bits; latency at one keyframe (3.1 to 4.2 us).
+// a lane cover the halves of a 128-byte line, so four lanes fetch whole lines; 16 lanes per pixel would pay more for joining and writing.
+// Bound: memory from about 64 float32 planes on (16 x 64 x 120 x 160, 4 alternatives: 21.2 us, 4.7 TB/s).  Below, memory and the vector
+// instructions of joining and writing a pixel together (8 x 32 x 120 x 160: 9.9 us, memory 6.2, 350 instructions a wave 5.6); in float16
+// vector instructions (16 x 64 x 120 x 160: 21.3 us, 535 a wave 17.3, memory 12.5); latency at one keyframe (3.6 to 4.8 us).
 template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_stats_last_kernel(PlaneFwd a) {
   constexpr int G = 4, N = 8;
@@ -613,7 +616,7 @@ struct Pull {
 };
 
 // neighbouring pixels next to each other: one lane per pixel and 16 planes, blockIdx.y numbers the groups of planes
-// Bound: memory (float16, 16 x 64 x 96 x 128: 13.4 us, 4.1 TB/s with the pixels' statistics read once per 16 planes)
+// Bound: memory (float16, 16 x 64 x 96 x 128: 13.0 us, 4.3 TB/s of what has to move; the pixels' statistics are read once per 16 planes)
 template <typename T, int K, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
   const uint32_t p = blockIdx.x * 256u + threadIdx.x;
@@ -637,7 +640,7 @@ __global__ void __launch_bounds__(256) plane_grad_first_kernel(PlaneBwd a) {
 }
 
 // the planes of a pixel next to each other, in the volume and in its gradient: four lanes per pixel, 16 bytes per lane, load and store
-// Bound: memory (4 x 256 x 120 x 160, mask, 4 alternatives: 37.8 us, 4.8 TB/s)
+// Bound: memory (4 x 256 x 120 x 160, mask, 4 alternatives: 37.7 us, 4.8 TB/s)
 template <typename T, int K, MaskKind M, typename Off>
 __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
   constexpr int G = 4, N = 8;
@@ -677,8 +680,9 @@ __global__ void __launch_bounds__(256) plane_grad_last_kernel(PlaneBwd a) {
 // ---- planes of depths ------------------------------------------------------------------------------------------------------------
 // 64-bit differences of 32-bit depths are exact within a factor of 2^29 (24 + 29 = 53 bits), so a tie is a tie there; beyond, rounding keeps
 // the order of the differences but may make equal ones of them.  16 planes' loads are in flight together.
-// Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 4.6 us, 5.1 with four waves).
-// Bound: memory where planes vary over the image (8 x 96 x 240 x 320: 46 us, 5.2 TB/s, a part from the last-level cache), else latency.
+// Workgroups of one wave: a keyframe's 300 waves spread over all compute units (19200 pixels, 64 planes: 4.7 us, 5.1 with four waves).
+// Bound: memory where planes vary over the image (8 x 96 x 240 x 320: 46.7 us, 5.2 TB/s, a part from the last-level cache; with four waves
+// 44.3), else latency.
 __global__ void __launch_bounds__(64) nearest_planes_kernel(PlaneNear a) {
   const uint32_t p = blockIdx.x * 64u + threadIdx.x;
   if (p >= (uint32_t)a.b * a.h * a.w) return;
@@ -745,9 +749,9 @@ void launch_stats(const PlaneFwd& a, hipStream_t s) {
   const dim3 block(256), by_pixel((pixels + 255) / 256), by_four((pixels + 63) / 64);
   // Four waves per 64 pixels pay (the exchange, four lanes writing a pixel) where few pixels with many planes would leave the chip idle.
   // Measured us, fp32, 0 / 4 alternatives, four waves against one:
-  //   D = 16:   19200 pixels  3.6 /  4.3 against  2.8 /  3.5; 307200 pixels 13.0 / 18.5 against  6.4 /  9.2
-  //   D = 64:   76800 pixels  6.3 /  8.7 against  7.1 / 10.5; 307200 pixels 15.5 / 22.7 against 17.0 / 21.1
-  //   D = 128: 153600 pixels 15.4 / 20.0 against 15.5 / 23.2; 307200 pixels 32.9 / 39.4 against 32.9 / 36.7
+  //   D = 16:   19200 pixels  4.2 /  4.9 against  3.2 /  4.2; 307200 pixels 13.8 / 19.8 against  6.3 / 10.0
+  //   D = 64:   76800 pixels  6.7 /  9.1 against  7.1 / 10.8; 307200 pixels 17.0 / 24.3 against 17.0 / 21.1
+  //   D = 128: 153600 pixels 15.4 / 21.2 against 15.7 / 24.2; 307200 pixels 32.0 / 41.1 against 31.8 / 39.7
   const bool share = (int64_t)pixels < 2400 * ((int64_t)a.d - 24);
   if (a.vs[1] == 1)
     by_mask(a.mask, a.ms[1], [&](auto m) { DT_LAUNCH((plane_stats_last_kernel<T, K, m.value, uint32_t>), by_four, block, 0, s, a); });
@@ -755,6 +759,9 @@ void launch_stats(const PlaneFwd& a, hipStream_t s) {
   else DT_LAUNCH((plane_stats_first_kernel<T, K, 1, uint32_t>), by_pixel, block, 0, s, a);
 }
 
+// Volumes, masks or outputs beyond 32-bit offsets: one kernel per layout and kind of mask, with 8 slots whatever top is.  Per byte that costs
+// little with alternatives and more without: float16, 57 x 128 x 480 x 640 (4.5 GB) against 48 of them (3.8 GB) with 32-bit offsets, us
+// per batch element: pixels innermost 29.1 against 25.4 with 4, 27.7 against 17.4 without; planes innermost 33.8 / 27.6 and 31.9 / 17.9.
 template <typename T>
 void launch_stats_wide(const PlaneFwd& a, hipStream_t s) {
   const uint32_t pixels = (uint32_t)a.b * a.h * a.w;
