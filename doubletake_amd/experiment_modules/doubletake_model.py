@@ -339,7 +339,8 @@ class _HotPathDepthModel(nn.Module):
         ``CostVolumeManager.plane_statistics(..., mask_bdhw=)``; in the loops ``mask_pred_depth`` drops the others.
 
         ``scale``: factor on the volume's scores in front of the softmax.  Two more launches per call; works under captured graphs and
-        launch programs, and for a driver of the two stages (volume_stage then returns the depth planes too).  ``loops`` can mask depths by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
+        launch programs, and for a driver of the two stages (volume_stage then returns the depth planes too).  ``loops`` can mask depths
+        by plane_log_prob_bhw (min_plane_log_prob=) before they are fused."""
         top, scale = int(top), float(scale)
         if on and not 0 <= top <= min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins):
             raise ValueError(f"top={top} not in 0..{min(plane_ops.MAX_TOP, self.cost_volume.num_depth_bins)}")

@@ -185,9 +185,11 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         are returned too.
     outside: log probability of a plane index outside 0..D-1: 0 drops such pixels out of a loss, -inf says that no plane is certain there.
 
-    Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice, not in forward mode): the gradient has the volume's
-    type and layout.  A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on
-    the current stream (planes innermost: one per 2^29 pixels) and can be captured into a graph; capture a backward pass only together with its forward pass."""
+    Differentiable in the volume (gradients of log_prob, entropy, log_sum and top_log_prob; not twice, not in forward mode): the
+    gradient has the volume's type and layout.  It is for a caller's own differentiable volume: the managers' volumes carry no graph.
+    A visible NaN or +inf makes the pixel's statistics NaN.  The call allocates its outputs, launches one kernel on the current stream
+    (planes innermost: one per 2^29 pixels) and can be captured into a graph; capture a backward pass only together with its forward
+    pass."""
     vol = volume_bdhw
     if vol.dim() != 4:
         raise ValueError(f"volume_bdhw must be [b, D, h, w], got {tuple(vol.shape)}")
@@ -236,10 +238,11 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
 
 @torch.no_grad()
 def nearest_planes(depth_bhw, depth_planes_bdhw):
-    """int64 [b, h, w]: index of the depth plane nearest to each depth (absolute difference, the lowest index of equally near ones), the depths taken in
-    float32 and the differences in float64: exact within a factor of 2^29, beyond it planes whose distances round to the same number are
-    equally near (all planes of a few metres to a depth of 1e20: plane 0); -1 where the depth is not finite or not positive (holes of a sensor's map, a renderer's background).  depth_planes_bdhw is
-    float32 and broadcastable to [b, D, h, w] (what the cost-volume managers return)."""
+    """int64 [b, h, w]: index of the depth plane nearest to each depth (absolute difference, the lowest index of equally near ones), the
+    depths taken in float32 and the differences in float64: exact within a factor of 2^29, beyond it planes whose distances round to the
+    same number are equally near (all planes of a few metres to a depth of 1e20: plane 0).  -1 where the depth is not finite or not
+    positive (holes of a sensor's map, a renderer's background).  depth_planes_bdhw is float32 and broadcastable to [b, D, h, w] (what
+    the cost-volume managers return)."""
     depth, planes = depth_bhw, depth_planes_bdhw
     if depth.dim() != 3:
         raise ValueError(f"depth_bhw must be [b, h, w], got {tuple(depth.shape)}")
