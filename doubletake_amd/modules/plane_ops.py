@@ -55,6 +55,11 @@ def _refuse_tangent(t, name):
         raise NotImplementedError(f"{name} carries a forward-mode tangent: plane_ops has reverse-mode gradients only")
 
 
+def _values(t):
+    """``t`` with its values in memory: the imaginary part of a conjugate is a view that torch negates when it is read."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _broadcast(t, shape, device, name):
     """``t`` as a view of ``shape`` = (b, D, h, w) with stride 0 along the axes it is broadcast over."""
     if t.device != device:
@@ -107,9 +112,9 @@ def _forward(vol, plane, top, scale, mask, planes, outside, for_grad):
 
 
 def _dense_f32(g):
-    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous() and not g.is_neg()):
         return g
-    return g.to(torch.float32).contiguous()
+    return _values(g).to(torch.float32).contiguous()
 
 
 def _check_saved(ctx, vol, plane, mask, ent, tpl):
@@ -231,6 +236,7 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         planes = _broadcast(planes, vol.shape, vol.device, "depth_planes_bdhw")
     _refuse_tangent(vol, "volume_bdhw")
     _require_gpu(vol, "volume_bdhw")
+    vol, planes = _values(vol), None if planes is None else _values(planes)
     if vol.requires_grad and torch.is_grad_enabled():
         return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes, outside))
     return _forward(vol, plane, top, scale, mask, planes, outside, False)[0]
@@ -256,7 +262,7 @@ def nearest_planes(depth_bhw, depth_planes_bdhw):
     D = planes.shape[1]
     if b * h * w >= 2**31 - 1:
         raise ValueError(f"depth_bhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
-    planes = _broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw")
+    planes = _values(_broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw"))
     _require_gpu(depth, "depth_bhw")
     depth = _dense_f32(depth)
     out = torch.empty((b, h, w), device=depth.device, dtype=torch.int64)

@@ -344,3 +344,11 @@ def test_header_states_which_outputs_go_together():
     for says in ("log_prob [b,h,w] goes with plane_bhw: both or neither", "top_log_prob and top_plane [b,top,h,w] are both required",
                  "top_depth [b,top,h,w] may be NULL and needs depth_planes", "row_max and row_log [b,h,w], both or neither"):
         assert says in words, says
+
+
+def test_gradients_that_torch_negates_when_read():
+    g = torch.tensor([[[2.0]]])
+    lazy = torch.complex(torch.zeros_like(g), -g).conj().imag
+    assert lazy.is_neg() and lazy.is_contiguous()
+    got = plane_ops._dense_f32(lazy)
+    assert not got.is_neg() and torch.equal(got, g) and plane_ops._dense_f32(g) is g and plane_ops._dense_f32(None) is None

@@ -661,3 +661,24 @@ def test_nearest_planes_of_far_depths(order):
         assert at == rounded.index(min(rounded)), float(z)
     if order == "ascending":
         assert got[:7] == [0, got[1], 32, 32, 32, 32, 32] and got[-6:] == [0] * 6
+
+
+@pytest.mark.parametrize("shape", [(2, 20, 5, 7), (1, 3, 1, 1)], ids=str)
+def test_views_that_torch_negates_when_read(shape):
+    """The imaginary part of a conjugate: what lies in memory has the other sign."""
+    vol, m, plane, planes = make(shape, mask="plane", seed=49)
+    lazy = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert lazy(vol).is_neg() and torch.equal(lazy(vol), vol)
+    kw = dict(top=2, mask_bdhw=m)
+    want = plane_ops.plane_log_probs(vol, plane, depth_planes_bdhw=planes, **kw)
+    got = plane_ops.plane_log_probs(lazy(vol), plane, depth_planes_bdhw=lazy(planes), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    depth = torch.rand(vol[:, 0].shape, generator=torch.Generator().manual_seed(1)).add(0.2).to(DEV)
+    assert torch.equal(plane_ops.nearest_planes(lazy(depth), lazy(planes)), plane_ops.nearest_planes(depth, planes))
+    grads = []
+    for f in (lambda t: t, lazy):
+        leaf = vol.detach().requires_grad_(True)
+        r = plane_ops.plane_log_probs(f(leaf), plane, **kw)
+        gs = [f(torch.full_like(r.entropy_bhw, v)) for v in (1.0, 0.5)]
+        grads.append(torch.autograd.grad([r.entropy_bhw, r.log_sum_bhw], leaf, gs)[0])
+    assert torch.equal(grads[0], grads[1])
