@@ -50,14 +50,8 @@ def _require_gpu(t, name):
 
 
 def _refuse_tangent(t, name):
-    # (a comparison outside forward mode: unpack_dual costs 3 us)
-    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+    if _forward_ad.unpack_dual(t).tangent is not None:
         raise NotImplementedError(f"{name} carries a forward-mode tangent: plane_ops has reverse-mode gradients only")
-
-
-def _values(t):
-    """``t`` with its values in memory: the imaginary part of a conjugate is a view that torch negates when it is read."""
-    return t.resolve_neg() if t.is_neg() else t
 
 
 def _broadcast(t, shape, device, name):
@@ -71,22 +65,22 @@ def _broadcast(t, shape, device, name):
     return t.expand(shape)
 
 
-def _desc(vol, top, scale, mask, planes, grad=None, outside=0.0):
+def _desc(vol, top, scale, mask, planes, outside=0.0):
     d = _abi.PlaneDesc()
     d.b, d.d, d.h, d.w = vol.shape
-    d.dtype, d.top, d.scale, d.outside = _DTYPES[vol.dtype], top, scale, outside
+    d.dtype, d.top, d.scale = _DTYPES[vol.dtype], top, scale
+    if outside:
+        d.outside = outside
     d.vol_stride[:] = vol.stride()
     if mask is not None:
         d.mask_stride[:] = mask.stride()
     if planes is not None:
         d.planes_stride[:] = planes.stride()
-    if grad is not None:
-        d.grad_stride[:] = grad.stride()
     return d
 
 
 def _forward(vol, plane, top, scale, mask, planes, outside, for_grad):
-    """(outputs, row statistics [2, b, h, w] or None, stream)"""
+    """(outputs, row statistics [2, b, h, w] or None, descriptor, stream)"""
     b, _, h, w = vol.shape
     ent = torch.empty((b, h, w), device=vol.device, dtype=torch.float32)
     lsum = torch.empty_like(ent)
@@ -103,47 +97,60 @@ def _forward(vol, plane, top, scale, mask, planes, outside, for_grad):
         rmax = rows.data_ptr()
         rlog = rmax + 4 * b * h * w
     stream = _abi.current_stream(vol.device)
+    desc = _desc(vol, top, scale, mask, planes, outside)
     if b * h * w:
         p = _abi.ptr
         _abi.check(_abi.lib().dt_cv_plane_log_probs(
-            _desc(vol, top, scale, mask, planes, None, outside), vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
+            desc, vol.data_ptr(), p(mask), p(plane), p(planes), p(lp), ent.data_ptr(), lsum.data_ptr(), p(tlp), p(tpl), p(tdep), rmax, rlog,
             stream), "dt_cv_plane_log_probs")
-    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, stream
+    return PlaneLogProbs(lp, ent, lsum, tlp, tpl, tdep), rows, desc, stream
 
 
 def _dense_f32(g):
-    if g is None or (g.dtype == torch.float32 and g.is_contiguous() and not g.is_neg()):
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous() and not g.is_neg()):
         return g
-    return _values(g).to(torch.float32).contiguous()
+    return g.to(torch.float32).resolve_neg().contiguous()
 
 
-def _check_saved(ctx, vol, plane, mask, ent, tpl):
-    """Hooks on saved tensors may bring a tensor back in another layout than it was saved in, which is fine, but also on another device
-    or of another type or size, and the kernel is given addresses: refused here.  (Written out: as a loop over the five it cost 2.3 us of
-    every gradient call, now 1.5.)"""
-    dev, shape = ctx.rows.device, ctx.shape
-    n = ctx.rows.numel() // 2
+def _refuse_saved(ctx, *saved):
+    back = [f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in saved if t is not None]
+    raise RuntimeError(f"a hook on saved tensors brought one back on another device, of another type or size than it was saved with "
+                       f"({ctx.dtype} {tuple(ctx.shape)} on {ctx.rows.device}): {'; '.join(back)}")
+
+
+def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
+    vol, plane, mask, ent, tpl = ctx.saved_tensors
+    rows, shape = ctx.rows, ctx.shape
+    dev, n = rows.device, rows.numel() // 2
+    # Hooks on saved tensors may bring a tensor back in another layout than it was saved in, which is fine, but also on another device or
+    # of another type or size, and the kernel is given addresses: refused.  (Written out: as a loop it cost 2.3 us of every call.)
     if (vol.device != dev or vol.dtype is not ctx.dtype or vol.shape != shape
             or ent.device != dev or ent.dtype is not torch.float32 or ent.numel() != n
             or (plane is not None and (plane.device != dev or plane.dtype is not torch.int64 or plane.numel() != n))
             or (mask is not None and (mask.device != dev or mask.dtype is not torch.bool or mask.shape != shape))
             or (tpl is not None and (tpl.device != dev or tpl.dtype is not torch.int64 or tpl.numel() != n * ctx.top))):
-        back = [f"{t.dtype} {tuple(t.shape)} on {t.device}" for t in (vol, plane, mask, ent, tpl) if t is not None]
-        raise RuntimeError(f"a hook on saved tensors brought one back on another device, of another type or size than it was saved with "
-                           f"({ctx.dtype} {tuple(shape)} on {dev}): {'; '.join(back)}")
-
-
-def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
-    vol, plane, mask, ent, tpl = ctx.saved_tensors
-    _check_saved(ctx, vol, plane, mask, ent, tpl)
-    g_lp, g_ent, g_lsum, g_top = _dense_f32(g_lp), _dense_f32(g_ent), _dense_f32(g_lsum), _dense_f32(g_top)
+        _refuse_saved(ctx, vol, plane, mask, ent, tpl)
+    if g_lp is not None:
+        g_lp = _dense_f32(g_lp)
+    if g_ent is not None:
+        g_ent = _dense_f32(g_ent)
+    if g_lsum is not None:
+        g_lsum = _dense_f32(g_lsum)
+    if g_top is not None:
+        g_top = _dense_f32(g_top)
     grad = torch.empty_like(vol)   # (dense, in the order of the volume's own strides)
-    n = ent.numel()
     if n:
-        # (strides are taken here: hooks on saved tensors may bring a tensor back in another layout than it was saved in)
-        p, desc = _abi.ptr, _desc(vol, ctx.top, ctx.scale, mask, None, grad)
-        plane, ent, tpl = [t if t is None or t.is_contiguous() else t.contiguous() for t in (plane, ent, tpl)]
-        rmax = ctx.rows.data_ptr()
+        p, desc = _abi.ptr, ctx.desc
+        if vol.stride() != ctx.vol_stride or (mask is not None and mask.stride() != ctx.mask_stride):
+            desc = _desc(vol, ctx.top, ctx.scale, mask, None)
+        desc.grad_stride[:] = grad.stride()
+        if not ent.is_contiguous():
+            ent = ent.contiguous()
+        if plane is not None and not plane.is_contiguous():
+            plane = plane.contiguous()
+        if tpl is not None and not tpl.is_contiguous():
+            tpl = tpl.contiguous()
+        rmax = rows.data_ptr()
         _abi.check(_abi.lib().dt_cv_plane_log_probs_grad(
             desc, vol.data_ptr(), p(mask), p(plane), ent.data_ptr(), p(tpl), rmax, rmax + 4 * n, p(g_lp), p(g_ent), p(g_lsum), p(g_top),
             grad.data_ptr(), ctx.stream), "dt_cv_plane_log_probs_grad")
@@ -153,15 +160,16 @@ def _backward(ctx, g_lp, g_ent, g_lsum, g_top, _g_plane, _g_depth):
 class _PlaneLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, vol, plane, top, scale, mask, planes, outside):
-        out, rows, stream = _forward(vol, plane, top, scale, mask, planes, outside, True)
+        out, rows, ctx.desc, ctx.stream = _forward(vol, plane, top, scale, mask, planes, outside, True)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(*[t for t in out[4:] if t is not None])
         ctx.save_for_backward(vol, plane, mask, out[1], out[4])
         # made here, neither inputs nor outputs.  The engine runs a backward on the stream its forward ran on: the handle is kept, asking
         # for it in the engine's thread costs 6 us
-        ctx.rows, ctx.stream, ctx.top, ctx.scale = rows, stream, top, scale
-        ctx.dtype, ctx.shape = vol.dtype, vol.shape
+        ctx.rows, ctx.top, ctx.scale, ctx.dtype, ctx.shape = rows, top, scale, vol.dtype, vol.shape
+        # (the descriptor serves the backward too, unless a hook on saved tensors brings one back in another layout)
+        ctx.vol_stride, ctx.mask_stride = vol.stride(), None if mask is None else mask.stride()
         return tuple(out)
 
     @staticmethod
@@ -234,9 +242,14 @@ def plane_log_probs(volume_bdhw, plane_bhw=None, top=0, scale=1.0, mask_bdhw=Non
         if planes.dtype != torch.float32:
             raise ValueError(f"depth_planes_bdhw is {planes.dtype}; float32 expected")
         planes = _broadcast(planes, vol.shape, vol.device, "depth_planes_bdhw")
-    _refuse_tangent(vol, "volume_bdhw")
+    if _forward_ad._current_level >= 0:   # (one comparison outside forward mode: unpack_dual costs 3 us)
+        _refuse_tangent(vol, "volume_bdhw")
     _require_gpu(vol, "volume_bdhw")
-    vol, planes = _values(vol), None if planes is None else _values(planes)
+    # (the imaginary part of a conjugate is a view that torch negates when it is read; the kernels read memory)
+    if vol.is_neg():
+        vol = vol.resolve_neg()
+    if planes is not None and planes.is_neg():
+        planes = planes.resolve_neg()
     if vol.requires_grad and torch.is_grad_enabled():
         return PlaneLogProbs(*_PlaneLogProbsFn.apply(vol, plane, top, scale, mask, planes, outside))
     return _forward(vol, plane, top, scale, mask, planes, outside, False)[0]
@@ -262,7 +275,9 @@ def nearest_planes(depth_bhw, depth_planes_bdhw):
     D = planes.shape[1]
     if b * h * w >= 2**31 - 1:
         raise ValueError(f"depth_bhw has {b * h * w} pixels; fewer than 2^31 - 1 are supported")
-    planes = _values(_broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw"))
+    planes = _broadcast(planes, (b, D, h, w), depth.device, "depth_planes_bdhw")
+    if planes.is_neg():
+        planes = planes.resolve_neg()
     _require_gpu(depth, "depth_bhw")
     depth = _dense_f32(depth)
     out = torch.empty((b, h, w), device=depth.device, dtype=torch.int64)

@@ -195,7 +195,8 @@ def _saved(**kw):
     t = dict(vol=torch.zeros(b, D, h, w), plane=torch.zeros(b, h, w, dtype=torch.int64), mask=torch.ones(b, D, h, w, dtype=torch.bool),
              ent=torch.zeros(b, h, w), tpl=torch.zeros(b, top, h, w, dtype=torch.int64))
     ctx = types.SimpleNamespace(rows=torch.zeros(2, b, h, w), stream=None, top=top, scale=1.0, dtype=torch.float32,
-                                shape=t["vol"].shape)
+                                shape=t["vol"].shape, vol_stride=t["vol"].stride(), mask_stride=t["mask"].stride(),
+                                desc=plane_ops._desc(t["vol"], top, 1.0, t["mask"], None))
     t.update(kw)
     ctx.saved_tensors = tuple(t.values())
     return ctx
